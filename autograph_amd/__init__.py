@@ -8,9 +8,11 @@ from .layer import (  # noqa: F401
     Conv2,
     Dense,
     Flatten,
+    LayerNorm,
     LeNet5,
     LeNet5Trainer,
     MaxPool2,
+    MxDense,
     Relu,
     SGD,
     conv2_direct_forward,
@@ -24,6 +26,7 @@ from .tensor import (  # noqa: F401
     Device,
     Im2ColConv2Options,
     MaxPool2Options,
+    MxTensor,
     Tensor,
     branch,
     gemm,

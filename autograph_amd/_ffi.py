@@ -24,6 +24,7 @@ f32 = C.c_float
 _GEMM = [i64, i64, i64, f32, ptr, i64, i64, i64, ptr, i64, i64, i64, f32, ptr, i64, i64, i64]
 _GEMM_B = [i64, i64, i64, i64, f32, ptr, i64, i64, i64, i64, ptr, i64, i64, i64, i64, f32, ptr, i64, i64, i64, i64,
            ptr, i64, i64, C.c_int]
+_BIAS_ACT = [ptr, i64, i64, C.c_int]
 _CONV = [ptr, ptr] + [i64] * 12
 _POOL = [ptr, ptr] + [i64] * 7
 
@@ -112,6 +113,19 @@ SIGNATURES = {
     "agh_cross_entropy_loss_bf16": ([ptr, ptr, i64, i64, ptr], C.c_int),
     "agh_cross_entropy_backward_f32": ([ptr, ptr, f32, ptr, i64, i64], C.c_int),
     "agh_cross_entropy_backward_bf16": ([ptr, ptr, f32, ptr, i64, i64], C.c_int),
+    "agh_layer_norm_f32": ([ptr, ptr, ptr, f32, ptr, ptr, ptr, i64, i64], C.c_int),
+    "agh_layer_norm_bf16": ([ptr, ptr, ptr, f32, ptr, ptr, ptr, i64, i64], C.c_int),
+    "agh_layer_norm_backward_f32": ([ptr] * 8 + [i64, i64], C.c_int),
+    "agh_layer_norm_backward_bf16": ([ptr] * 8 + [i64, i64], C.c_int),
+    "agh_mxfp4_bytes": ([i64, i64, C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)], C.c_int),
+    "agh_quantize_mxfp4_f32": ([ptr] + [i64] * 5 + [ptr, ptr], C.c_int),
+    "agh_quantize_mxfp4_bf16": ([ptr] + [i64] * 5 + [ptr, ptr], C.c_int),
+    "agh_dequantize_mxfp4_f32": ([ptr, ptr, i64, i64, ptr, i64, i64, i64], C.c_int),
+    "agh_dequantize_mxfp4_bf16": ([ptr, ptr, i64, i64, ptr, i64, i64, i64], C.c_int),
+    "agh_gemm_mxfp4_f32": ([i64] * 3 + [ptr] * 5 + [i64] * 3 + _BIAS_ACT, C.c_int),
+    "agh_gemm_mxfp4_bf16": ([i64] * 3 + [ptr] * 5 + [i64] * 3 + _BIAS_ACT, C.c_int),
+    "agh_dense_mxfp4_f32": ([i64] * 3 + [ptr] + [i64] * 3 + [ptr] * 3 + [i64] * 3 + _BIAS_ACT, C.c_int),
+    "agh_dense_mxfp4_bf16": ([i64] * 3 + [ptr] + [i64] * 3 + [ptr] * 3 + [i64] * 3 + _BIAS_ACT, C.c_int),
     "agh_accuracy_f32": ([ptr, ptr, i64, i64, ptr], C.c_int),
     "agh_accuracy_bf16": ([ptr, ptr, i64, i64, ptr], C.c_int),
 }

@@ -30,6 +30,9 @@ namespace {
     X(agh_relu_f32) X(agh_relu_bf16) X(agh_relu_backward_f32) X(agh_relu_backward_bf16)                                                  \
     X(agh_assign_f32) X(agh_assign_bf16) X(agh_scaled_add_f32) X(agh_scaled_add_bf16)                                                    \
     X(agh_scaled_add_strided_f32) X(agh_scaled_add_strided_bf16) X(agh_sum_axis0_f32) X(agh_sum_axis0_bf16)                              \
+    X(agh_layer_norm_f32) X(agh_layer_norm_bf16) X(agh_layer_norm_backward_f32) X(agh_layer_norm_backward_bf16)                          \
+    X(agh_quantize_mxfp4_f32) X(agh_quantize_mxfp4_bf16) X(agh_dequantize_mxfp4_f32) X(agh_dequantize_mxfp4_bf16)                        \
+    X(agh_gemm_mxfp4_f32) X(agh_gemm_mxfp4_bf16) X(agh_dense_mxfp4_f32) X(agh_dense_mxfp4_bf16)                                          \
     X(agh_lenet5_forward_f32) X(agh_lenet5_forward_bf16) X(agh_memcpy_d2d) X(agh_graph_launch)
 
 // every entry point used here, as setup() has found it

@@ -163,6 +163,10 @@ class Dense:
             out.add_assign(self.bias)
         return out.relu() if relu else out
 
+    def quantize_mxfp4(self):
+        """The layer for inference with its weight in 4 bits."""
+        return MxDense(self.weight.quantize_mxfp4(axis=0), self.bias)
+
     def to_json(self):
         import json
         from . import serde
@@ -178,6 +182,50 @@ class Dense:
         layer = cls(_device_param(f["weight"], dtype), _device_param(f["bias"], dtype))
         layer.weight_state, layer.bias_state = _device_state(f["weight"]), _device_state(f["bias"])
         return layer
+
+
+class MxDense:
+    """`Dense` with its weight [inputs, outputs] in MXFP4, quantised along the inputs (`Dense.quantize_mxfp4`), and the bias as it was.  The
+    input is quantised along its rows at every call; the sums are f32, and the result is rounded once, after bias and relu."""
+
+    def __init__(self, weight, bias=None):
+        if weight.axis != 0:
+            raise AghError(-1, "MxDense: the weight must be quantised along axis 0, its inputs")
+        self.weight, self.bias = weight, bias
+
+    def forward(self, x, relu=False):
+        """The bits of `x.quantize_mxfp4().dot(weight, bias, relu, x.dtype)` in one call."""
+        if x.ndim != 2:
+            raise AghError(-1, "MxDense: the input must be 2-D")
+        (m, k), (k2, n) = x.shape, self.weight.shape
+        if k != k2:
+            raise AghError(-1, f"a_cols != b_rows, {k} != {k2}")
+        b = self.bias
+        if b is not None and (b.dtype != x.dtype or b.shape != (n,)):
+            raise AghError(-1, f"bias must be a {x.dtype} vector of length {n}")
+        y = Tensor.uninit((m, n), x.dtype)
+        bp, bo, bs_ = (b._ptr(), b.offset, b.strides[0]) if b is not None else (None, 0, 0)
+        x._call("agh_dense_mxfp4")(m, k, n, x._ptr(), x.offset, x.strides[0], x.strides[1], self.weight.codes.ptr, self.weight.scales.ptr, y._ptr(), 0, n, 1,
+                                   bp, bo, bs_, 1 if relu else 0)
+        return y
+
+
+class LayerNorm:
+    """Layer norm over the last axis: weight and bias [features], either None (no counterpart in the reference)."""
+
+    def __init__(self, weight=None, bias=None, epsilon=1e-5):
+        self.weight, self.bias, self.epsilon = weight, bias, epsilon
+
+    def forward(self, x):
+        return x.layer_norm(self.weight, self.bias, self.epsilon)
+
+    def forward_train(self, x):
+        """(y, mean, rstd): the statistics are what `backward` takes."""
+        return x.layer_norm(self.weight, self.bias, self.epsilon, stats=True)
+
+    def backward(self, x, output_grad, mean, rstd):
+        """(dx, dweight, dbias)."""
+        return x.layer_norm_backward(output_grad, self.weight, mean, rstd)
 
 
 class MaxPool2:

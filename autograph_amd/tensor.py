@@ -104,6 +104,10 @@ def _dims(shape):
     return dims
 
 
+def _ptr_or_none(t):
+    return None if t is None else t._data_ptr()
+
+
 def _std_strides(shape):
     if len(shape) == 2:
         return (shape[1], 1)
@@ -402,12 +406,149 @@ class Tensor:
         check(lib.agh_memcpy_d2h(out.ctypes.data, tmp.ptr, 4))
         return float(out[0])
 
+    # -- layer norm over the last axis (no counterpart in the reference) --
+    def _norm_vector(self, v, name):
+        if v is None:
+            return None
+        if v.dtype != self.dtype or v.shape != self.shape[-1:]:
+            raise AghError(-1, f"layer_norm: {name} must be a {self.dtype} vector of length {self.shape[-1]}")
+        return v.as_standard_layout()
+
+    def layer_norm(self, weight=None, bias=None, epsilon=1e-5, stats=False):
+        """(x - mean) / sqrt(var + epsilon) * weight + bias over the last axis.  With `stats`: (y, mean, rstd), the f32 tensors that
+        `layer_norm_backward` takes, one value a row."""
+        if self.ndim < 1:
+            raise AghError(-1, "layer_norm: a tensor without axes")
+        x = self.as_standard_layout()
+        w, b = self._norm_vector(weight, "weight"), self._norm_vector(bias, "bias")
+        lead = x.shape[:-1]
+        y = _uninit(x.shape, x.dtype)
+        mean, rstd = (_uninit(lead, F32), _uninit(lead, F32)) if stats else (None, None)
+        self._call("agh_layer_norm")(x._data_ptr(), _ptr_or_none(w), _ptr_or_none(b), epsilon, y._ptr(), _ptr_or_none(mean),
+                                     _ptr_or_none(rstd), math.prod(lead), x.shape[-1])
+        return (y, mean, rstd) if stats else y
+
+    def layer_norm_backward(self, output_grad, weight, mean, rstd):
+        """Gradients (dx, dweight, dbias) of `self.layer_norm(weight, bias, stats=True)`, `self` being its input; with weight None
+        (dx, None, None)."""
+        if self.ndim < 1:
+            raise AghError(-1, "layer_norm_backward: a tensor without axes")
+        if output_grad.dtype != self.dtype or output_grad.shape != self.shape:
+            raise AghError(-1, f"layer_norm_backward: expected a {self.dtype} gradient of {self.shape}, found {output_grad.dtype} {output_grad.shape}")
+        lead = self.shape[:-1]
+        for name, v in (("mean", mean), ("rstd", rstd)):
+            if v.dtype != F32 or v.shape != lead:
+                raise AghError(-1, f"layer_norm_backward: {name} must be an f32 tensor of {lead}, found {v.dtype} {v.shape}")
+        x, dy, mean, rstd = self.as_standard_layout(), output_grad.as_standard_layout(), mean.as_standard_layout(), rstd.as_standard_layout()
+        w = self._norm_vector(weight, "weight")
+        dx = _uninit(x.shape, x.dtype)
+        dw, db = (_uninit(x.shape[-1:], x.dtype), _uninit(x.shape[-1:], x.dtype)) if w is not None else (None, None)
+        self._call("agh_layer_norm_backward")(x._data_ptr(), dy._data_ptr(), _ptr_or_none(w), mean._data_ptr(), rstd._data_ptr(), dx._ptr(),
+                                              _ptr_or_none(dw), _ptr_or_none(db), math.prod(lead), x.shape[-1])
+        return dx, dw, db
+
+    # -- MXFP4 (no counterpart in the reference) --
+    def quantize_mxfp4(self, axis=1):
+        """The matrix in 4 bits, blocks of 32 along `axis`: the axis that a product will sum over (1 for a left operand, 0 for a right one)."""
+        if self.ndim != 2 or axis not in (0, 1):
+            raise AghError(-1, f"quantize_mxfp4: a matrix and axis 0 or 1 expected, found {self.shape} and {axis!r}")
+        out = MxTensor.uninit(self.shape, axis)
+        self._call("agh_quantize_mxfp4")(self._ptr(), self.offset, self.strides[1 - axis], self.strides[axis], self.shape[1 - axis], self.shape[axis],
+                                         out.codes.ptr, out.scales.ptr)
+        return out
+
     def cross_entropy_loss_backward(self, target, dy=1.0):
         x = self.as_standard_layout()
         bs, classes = x.shape
         dx = _uninit(x.shape, x.dtype)
         check(self._fn("agh_cross_entropy_backward")(x._data_ptr(), target.ptr, dy, dx._ptr(), bs, classes))
         return dx
+
+
+class MxTensor:
+    """A matrix in MXFP4: blocks of 32 values along `axis` share a scale, a power of two, and hold 4 bits each.  `codes` and `scales` are laid
+    out for the matrix cores (include/autograph_hip.h); `into_arrays` and `from_arrays` give and take them by rows."""
+
+    def __init__(self, codes, scales, shape, axis):
+        self.codes, self.scales, self.shape, self.axis = codes, scales, shape, axis
+
+    @classmethod
+    def uninit(cls, shape, axis):
+        rows, k = shape[1 - axis], shape[axis]
+        steps = -(-k // 128)
+        return cls(Buffer(-(-rows // 16) * steps * 1024), Buffer(-(-rows // 64) * steps * 256), shape, axis)
+
+    def t(self):
+        """The transposed matrix: no data moves, the blocks run along the other axis."""
+        return MxTensor(self.codes, self.scales, self.shape[::-1], 1 - self.axis)
+
+    def dequantize(self, dtype=F32):
+        """The values that the codes stand for; both types hold them exactly."""
+        if dtype not in _ITEMSIZE:
+            raise AghError(-1, f"dequantize: unknown type {dtype!r}")
+        y = _uninit(self.shape, dtype)
+        a = self.axis
+        y._call("agh_dequantize_mxfp4")(self.codes.ptr, self.scales.ptr, self.shape[1 - a], self.shape[a], y._ptr(), 0, y.strides[1 - a], y.strides[a])
+        return y
+
+    def dot(self, rhs, bias=None, relu=False, dtype=BF16):
+        """`Tensor.dot` of two quantised matrices, each along the axis that is summed over; bias and relu in the same launch, one rounding."""
+        if self.axis != 1 or rhs.axis != 0:
+            raise AghError(-1, "dot: the left operand must be quantised along axis 1 and the right one along axis 0, the axes that are summed over")
+        (m, k), (k2, n) = self.shape, rhs.shape
+        if k != k2:
+            raise AghError(-1, f"a_cols != b_rows, {k} != {k2}")
+        if dtype not in _ITEMSIZE:
+            raise AghError(-1, f"dot: unknown type {dtype!r}")
+        if bias is not None and (bias.dtype != dtype or bias.shape != (n,)):
+            raise AghError(-1, f"bias must be a {dtype} vector of length {n}")
+        out = _uninit((m, n), dtype)
+        bp, bo, bs_ = (bias._ptr(), bias.offset, bias.strides[0]) if bias is not None else (None, 0, 0)
+        out._call("agh_gemm_mxfp4")(m, k, n, self.codes.ptr, self.scales.ptr, rhs.codes.ptr, rhs.scales.ptr, out._ptr(), 0, n, 1, bp, bo, bs_, 1 if relu else 0)
+        return out
+
+    @staticmethod
+    def _places(rows, k):
+        """Byte offsets of [rows, blocks] in codes and scales."""
+        steps = -(-k // 128)
+        r, b = np.arange(rows, dtype=np.int64)[:, None], np.arange(-(-k // 32), dtype=np.int64)[None, :]
+        inner = b % 4 * 16 + r % 16
+        return ((r // 16 * steps + b // 4) * 64 + inner) * 16, ((r // 64 * steps + b // 4) * 64 + inner) * 4 + r // 16 % 4
+
+    def into_arrays(self):
+        """Blocking: (codes, scale bytes) as uint8, one code a byte in the matrix's own shape, scales with a block for 32 values of `axis`."""
+        rows, k = self.shape[1 - self.axis], self.shape[self.axis]
+        raw = []
+        for b in (self.codes, self.scales):
+            raw.append(np.empty(b.nbytes, np.uint8))
+            check(lib.agh_memcpy_d2h(raw[-1].ctypes.data, b.ptr, b.nbytes))
+        at_codes, at_scales = self._places(rows, k)
+        packed = raw[0][at_codes[..., None] + np.arange(16)]
+        codes = np.stack((packed & 15, packed >> 4), -1).reshape(rows, -1)[:, :k]
+        scales = raw[1][at_scales]
+        return (codes, scales) if self.axis == 1 else (np.ascontiguousarray(codes.T), np.ascontiguousarray(scales.T))
+
+    @classmethod
+    def from_arrays(cls, codes, scales, axis=1):
+        """The inverse: a matrix quantised elsewhere."""
+        codes, scales = np.asarray(codes), np.asarray(scales)
+        if codes.ndim != 2 or scales.ndim != 2 or axis not in (0, 1) or codes.dtype != np.uint8 or scales.dtype != np.uint8:
+            raise AghError(-1, "MxTensor.from_arrays: uint8 matrices of codes and scales and axis 0 or 1 expected")
+        out = cls.uninit(codes.shape, axis)
+        if axis == 0:
+            codes, scales = codes.T, scales.T
+        rows, k = codes.shape
+        if scales.shape != (rows, -(-k // 32)) or (codes > 15).any():
+            raise AghError(-1, f"MxTensor.from_arrays: codes below 16 and one scale for 32 of them expected, found {codes.shape} and {scales.shape}")
+        packed = np.zeros((rows, -(-k // 32), 32), np.uint8)
+        packed.reshape(rows, -1)[:, :k] = codes
+        at_codes, at_scales = cls._places(rows, k)
+        for b, at, values in ((out.codes, at_codes[..., None] + np.arange(16), packed[..., 0::2] | packed[..., 1::2] << 4), (out.scales, at_scales, scales)):
+            raw = np.zeros(b.nbytes, np.uint8)
+            raw[at] = values
+            check(lib.agh_memcpy_h2d(b.ptr, raw.ctypes.data, raw.nbytes))
+            check(lib.agh_sync())  # `raw` is a temporary
+        return out
 
 
 @contextlib.contextmanager

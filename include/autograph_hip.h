@@ -411,6 +411,78 @@ int agh_relu_bf16(const void *x, void *y, int64_t n);
 int agh_relu_backward_f32(const void *x, const void *dy, void *dx, int64_t n);
 int agh_relu_backward_bf16(const void *x, const void *dy, void *dx, int64_t n);
 
+/* -------------------------------------------------------------- layer norm ---- */
+
+/* Layer norm over the rows of x [rows, cols] in standard layout; no counterpart in the reference, it stands with the layers of
+ * src/learn/neural_network/layer.rs:
+ *   mean = sum x / cols, rstd = 1 / sqrt(sum (x - mean)^2 / cols + eps), y = (x - mean) * rstd * weight + bias
+ * weight and bias have cols elements of the same type; a null weight stands for ones, a null bias for zeros.  mean and rstd,
+ * rows floats each, are what the backward call takes; either may be null.  y may be x.  Sums are f32, y is rounded once.
+ * rows == 0 does nothing; cols must be at least 1, both below 2^31. */
+int agh_layer_norm_f32(const void *x, const void *weight, const void *bias, float eps, void *y, void *mean, void *rstd,
+                       int64_t rows, int64_t cols);
+int agh_layer_norm_bf16(const void *x, const void *weight, const void *bias, float eps, void *y, void *mean, void *rstd,
+                        int64_t rows, int64_t cols);
+
+/* Its gradients, h = (x - mean) * rstd and g = dy * weight:
+ *   dx = rstd * (g - sum g / cols - h * sum (g * h) / cols), dweight = sum over rows of dy * h, dbias = sum over rows of dy
+ * x, dy, dx: [rows, cols] in standard layout, dx may be x or dy; mean, rstd: as the forward call wrote them.  Each of dx, dweight
+ * and dbias may be null and is then not formed.  Sums are f32 and added in an order that depends on the sizes alone, results
+ * rounded once.  rows == 0 writes zeros to dweight and dbias.  Uses the library's workspace. */
+int agh_layer_norm_backward_f32(const void *x, const void *dy, const void *weight, const void *mean, const void *rstd,
+                                void *dx, void *dweight, void *dbias, int64_t rows, int64_t cols);
+int agh_layer_norm_backward_bf16(const void *x, const void *dy, const void *weight, const void *mean, const void *rstd,
+                                 void *dx, void *dweight, void *dbias, int64_t rows, int64_t cols);
+
+/* ------------------------------------------------------------------- MXFP4 ---- */
+
+/* Microscaled 4-bit floating point (MXFP4 of the OCP microscaling formats): blocks of 32 values along k share a scale 2^(s - 127), s one
+ * byte, 255 for NaN; each value is a code of 4 bits, sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6.  No counterpart in the reference;
+ * what `Tensor::dot` (src/tensor/linalg.rs:410-421) and `Dense` (layer.rs:1134-1143) do, on operands of a quarter of bf16's size.
+ *
+ * A matrix of `rows` rows of k values takes two buffers whose sizes agh_mxfp4_bytes says:
+ *   codes   16-byte aligned: the 32 codes of row r, block b (of 32 along k), the even k in the low half of a byte, are the 16 bytes at
+ *           ((r / 16 * steps + b / 4) * 64 + b % 4 * 16 + r % 16) * 16, steps = ceil(k / 128)
+ *   scales  4-byte aligned: their byte is at ((r / 64 * steps + b / 4) * 64 + b % 4 * 16 + r % 16) * 4 + r / 16 % 4
+ * Values behind k are zeros: codes 0, and the scale byte 0 where a whole block lies behind k; the last 128 of a row are always whole.
+ * Rows behind the last one (r up to a multiple of 16, of 64 for the scales) may hold anything. */
+int agh_mxfp4_bytes(int64_t rows, int64_t k, size_t *codes, size_t *scales);
+
+/* x [rows, k] with element strides rs, cs (any; blocks run along k, so the transposed view of a matrix quantises it along its columns):
+ *   s = max(0, min(254, 127 + floor(log2(largest magnitude of the block)) - 2)), code = x / 2^(s - 127) to the nearest, half to even, above 6 to 6
+ * A block that holds an infinity or a NaN gets s = 255: it stands for NaNs. */
+int agh_quantize_mxfp4_f32(const void *x, int64_t off_x, int64_t rs, int64_t cs, int64_t rows, int64_t k, void *codes,
+                           void *scales);
+int agh_quantize_mxfp4_bf16(const void *x, int64_t off_x, int64_t rs, int64_t cs, int64_t rows, int64_t k, void *codes,
+                            void *scales);
+/* The values that the codes stand for (exact in either type) into y [rows, k] with element strides rs, cs, whose elements must be
+ * distinct addresses. */
+int agh_dequantize_mxfp4_f32(const void *codes, const void *scales, int64_t rows, int64_t k, void *y, int64_t off_y,
+                             int64_t rs, int64_t cs);
+int agh_dequantize_mxfp4_bf16(const void *codes, const void *scales, int64_t rows, int64_t k, void *y, int64_t off_y,
+                              int64_t rs, int64_t cs);
+
+/* c[off_c + i*rsc + j*csc] = act(sum_x a[i][x] * b[j][x] + bias[off_bias + j*bias_stride]), i < m, j < n: a [m, k] and b [n, k] quantised, both
+ * along k.  Sums are f32 on the matrix cores, bias (may be null) and act are applied in f32 and the result is rounded once.  c must not overlap
+ * the operands and its elements must be distinct addresses; m, n or k == 0 is allowed (k == 0 yields act(bias)).  May use the library's
+ * workspace. */
+int agh_gemm_mxfp4_f32(int64_t m, int64_t k, int64_t n, const void *a_codes, const void *a_scales, const void *b_codes,
+                       const void *b_scales, void *c, int64_t off_c, int64_t rsc, int64_t csc,
+                       const void *bias, int64_t off_bias, int64_t bias_stride, int act);
+int agh_gemm_mxfp4_bf16(int64_t m, int64_t k, int64_t n, const void *a_codes, const void *a_scales, const void *b_codes,
+                        const void *b_scales, void *c, int64_t off_c, int64_t rsc, int64_t csc,
+                        const void *bias, int64_t off_bias, int64_t bias_stride, int act);
+
+/* Dense forward with a quantised weight: x [m, k] (element strides rsx, csx) is quantised along k as agh_quantize_mxfp4_<T> does and multiplied with
+ * w, the weight [k, n] quantised along k (n rows of k values, as agh_quantize_mxfp4_<T> writes them from the transposed view).  The same bits as
+ * the two calls.  Uses the library's workspace. */
+int agh_dense_mxfp4_f32(int64_t m, int64_t k, int64_t n, const void *x, int64_t off_x, int64_t rsx, int64_t csx,
+                        const void *w_codes, const void *w_scales, void *c, int64_t off_c, int64_t rsc, int64_t csc,
+                        const void *bias, int64_t off_bias, int64_t bias_stride, int act);
+int agh_dense_mxfp4_bf16(int64_t m, int64_t k, int64_t n, const void *x, int64_t off_x, int64_t rsx, int64_t csx,
+                         const void *w_codes, const void *w_scales, void *c, int64_t off_c, int64_t rsc, int64_t csc,
+                         const void *bias, int64_t off_bias, int64_t bias_stride, int act);
+
 /* ---- around the contraction path: what a training step needs besides the ops above ----
  * All follow the HOST arithmetic of the reference: every operation the host performs in the
  * element type is rounded to the element type, sums run in the host's order. */

@@ -88,6 +88,19 @@ extern "C" {
     pub fn agh_relu_bf16(x: *const c_void, y: *mut c_void, n: i64) -> c_int;
     pub fn agh_relu_backward_f32(x: *const c_void, dy: *const c_void, dx: *mut c_void, n: i64) -> c_int;
     pub fn agh_relu_backward_bf16(x: *const c_void, dy: *const c_void, dx: *mut c_void, n: i64) -> c_int;
+    pub fn agh_layer_norm_f32(x: *const c_void, weight: *const c_void, bias: *const c_void, eps: f32, y: *mut c_void, mean: *mut c_void, rstd: *mut c_void, rows: i64, cols: i64) -> c_int;
+    pub fn agh_layer_norm_bf16(x: *const c_void, weight: *const c_void, bias: *const c_void, eps: f32, y: *mut c_void, mean: *mut c_void, rstd: *mut c_void, rows: i64, cols: i64) -> c_int;
+    pub fn agh_layer_norm_backward_f32(x: *const c_void, dy: *const c_void, weight: *const c_void, mean: *const c_void, rstd: *const c_void, dx: *mut c_void, dweight: *mut c_void, dbias: *mut c_void, rows: i64, cols: i64) -> c_int;
+    pub fn agh_layer_norm_backward_bf16(x: *const c_void, dy: *const c_void, weight: *const c_void, mean: *const c_void, rstd: *const c_void, dx: *mut c_void, dweight: *mut c_void, dbias: *mut c_void, rows: i64, cols: i64) -> c_int;
+    pub fn agh_mxfp4_bytes(rows: i64, k: i64, codes: *mut usize, scales: *mut usize) -> c_int;
+    pub fn agh_quantize_mxfp4_f32(x: *const c_void, off_x: i64, rs: i64, cs: i64, rows: i64, k: i64, codes: *mut c_void, scales: *mut c_void) -> c_int;
+    pub fn agh_quantize_mxfp4_bf16(x: *const c_void, off_x: i64, rs: i64, cs: i64, rows: i64, k: i64, codes: *mut c_void, scales: *mut c_void) -> c_int;
+    pub fn agh_dequantize_mxfp4_f32(codes: *const c_void, scales: *const c_void, rows: i64, k: i64, y: *mut c_void, off_y: i64, rs: i64, cs: i64) -> c_int;
+    pub fn agh_dequantize_mxfp4_bf16(codes: *const c_void, scales: *const c_void, rows: i64, k: i64, y: *mut c_void, off_y: i64, rs: i64, cs: i64) -> c_int;
+    pub fn agh_gemm_mxfp4_f32(m: i64, k: i64, n: i64, a_codes: *const c_void, a_scales: *const c_void, b_codes: *const c_void, b_scales: *const c_void, c: *mut c_void, off_c: i64, rsc: i64, csc: i64, bias: *const c_void, off_bias: i64, bias_stride: i64, act: c_int) -> c_int;
+    pub fn agh_gemm_mxfp4_bf16(m: i64, k: i64, n: i64, a_codes: *const c_void, a_scales: *const c_void, b_codes: *const c_void, b_scales: *const c_void, c: *mut c_void, off_c: i64, rsc: i64, csc: i64, bias: *const c_void, off_bias: i64, bias_stride: i64, act: c_int) -> c_int;
+    pub fn agh_dense_mxfp4_f32(m: i64, k: i64, n: i64, x: *const c_void, off_x: i64, rsx: i64, csx: i64, w_codes: *const c_void, w_scales: *const c_void, c: *mut c_void, off_c: i64, rsc: i64, csc: i64, bias: *const c_void, off_bias: i64, bias_stride: i64, act: c_int) -> c_int;
+    pub fn agh_dense_mxfp4_bf16(m: i64, k: i64, n: i64, x: *const c_void, off_x: i64, rsx: i64, csx: i64, w_codes: *const c_void, w_scales: *const c_void, c: *mut c_void, off_c: i64, rsc: i64, csc: i64, bias: *const c_void, off_bias: i64, bias_stride: i64, act: c_int) -> c_int;
     pub fn agh_assign_f32(x: *const c_void, off_x: i64, sx0: i64, sx1: i64, sx2: i64, sx3: i64, y: *mut c_void, off_y: i64, sy0: i64, sy1: i64, sy2: i64, sy3: i64, d0: i64, d1: i64, d2: i64, d3: i64) -> c_int;
     pub fn agh_assign_bf16(x: *const c_void, off_x: i64, sx0: i64, sx1: i64, sx2: i64, sx3: i64, y: *mut c_void, off_y: i64, sy0: i64, sy1: i64, sy2: i64, sy3: i64, d0: i64, d1: i64, d2: i64, d3: i64) -> c_int;
     pub fn agh_scaled_add_f32(y: *mut c_void, alpha: f32, x: *const c_void, n: i64) -> c_int;
