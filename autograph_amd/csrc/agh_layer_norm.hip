@@ -3,43 +3,348 @@
 //   mean = sum x / C, rstd = 1 / sqrt(sum (x - mean)^2 / C + eps), y = (x - mean) rstd w + b
 //   with h = (x - mean) rstd and g = dy w:  dx = rstd (g - sum g / C - h sum (g h) / C), dw = sum over rows dy h, db = sum over rows dy
 // All sums are f32, whatever the element type, and every result is rounded to it once.
+//
+// Bounded by memory: each element is read once and written once.  A row stays in the registers of the threads that share it, in 16-byte
+// groups, between its sums and its result; so the squares can be taken of deviations from the finished mean.  Up to 8 groups a lane a row belongs to
+// one wave, whose sums need neither LDS nor a barrier, longer ones to a workgroup.  Threads keep their columns from row to row: weight and bias are read
+// once, and the backward pass adds its columns' shares of dw and db in registers.
 #include "agh_internal.h"
 
 using namespace agh;
 
 namespace {
 
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
 constexpr int kThreads = 256;
 
-// sum over the workgroup, the same bits in every thread; `part`: one f32 a wave
-__device__ __forceinline__ float workgroup_sum(float v, float *part) {
+// sum over TPR neighbouring lanes (16 or 64), the same bits in each of them
+template <int TPR>
+__device__ __forceinline__ float lanes_sum(float v) {
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xF, 0xF, true));   // quad_perm 1 0 3 2
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xF, 0xF, true));   // quad_perm 2 3 0 1
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xF, 0xF, true));  // row_half_mirror
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xF, 0xF, true));  // row_mirror
+    if constexpr (TPR == 64) {
+        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+        v = __int_as_float(a[0]) + __int_as_float(a[1]);
+        const auto b = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+        v = __int_as_float(b[0]) + __int_as_float(b[1]);
+    }
+    return v;
+}
+
+// N sums over the TPR threads of a row; beyond a wave through `part` (N floats a wave, not the memory of the sums before: its readers may still be at it)
+template <int TPR, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], float *part) {
 #pragma unroll
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+    for (int i = 0; i < N; ++i) v[i] = lanes_sum<(TPR < 64 ? TPR : 64)>(v[i]);
+    if constexpr (TPR > 64) {
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int i = 0; i < N; ++i) part[(threadIdx.x >> 6) * N + i] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float s = 0.0f;
+#pragma unroll
+            for (int j = 0; j < TPR / 64; ++j) s += part[j * N + i];
+            v[i] = s;
+        }
+    }
+}
+
+template <typename T> struct Unaligned;
+template <> struct Unaligned<float> { typedef u32x4_t vec __attribute__((aligned(4))); };
+template <> struct Unaligned<uint16_t> { typedef u32x4_t vec __attribute__((aligned(2))); };
+
+// 16 bytes of a row from element e on, at any element's address; zeros behind its end
+template <typename T>
+struct Group {
+    static constexpr int VE = 16 / (int)sizeof(T);
+    typedef typename Unaligned<T>::vec vec;
+    union Bits { u32x4_t q; T e[VE]; };
+    static __device__ __forceinline__ u32x4_t load(const T *row, int e, int cols) {
+        if (e + VE <= cols) return *(const vec *)(row + e);
+        Bits b;
+        b.q = u32x4_t{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < VE; ++i)
+            if (e + i < cols) b.e[i] = row[e + i];
+        return b.q;
+    }
+    // the elements of a weight that may be absent: `none` is what it stands for then
+    static __device__ __forceinline__ u32x4_t load_or(const T *row, int e, int cols, float none) {
+        if (row) return load(row, e, cols);
+        float f[VE];
+#pragma unroll
+        for (int i = 0; i < VE; ++i) f[i] = none;
+        return pack(f);
+    }
+    static __device__ __forceinline__ void store(T *row, int e, int cols, u32x4_t v) {
+        if (e + VE <= cols) {
+            *(vec *)(row + e) = v;
+            return;
+        }
+        Bits b;
+        b.q = v;
+#pragma unroll
+        for (int i = 0; i < VE; ++i)
+            if (e + i < cols) row[e + i] = b.e[i];
+    }
+    static __device__ __forceinline__ float get(u32x4_t v, int i) {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(v[i]);
+        else return __uint_as_float(i & 1 ? v[i / 2] & 0xFFFF0000u : v[i / 2] << 16);
+    }
+    static __device__ __forceinline__ u32x4_t pack(const float (&f)[VE]) {
+        u32x4_t v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) v[i] = __float_as_uint(f[i]);
+            else v[i] = f32x2_to_bf16x2(f[2 * i], f[2 * i + 1]);
+        }
+        return v;
+    }
+};
+
+// Values that stay packed: without this the compiler widens them once for all their uses, which takes a bf16 row twice the registers
+__device__ __forceinline__ void keep_packed(u32x4_t &v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t w = v[i];
+        asm("" : "+v"(w));
+        v[i] = w;
+    }
+}
+
+constexpr int wg_threads(int tpr) { return tpr > kThreads ? tpr : kThreads; }
+
+// rows of at most TPR * VPT groups, TPR threads a row
+template <typename T, int TPR, int VPT>
+__global__ __launch_bounds__(wg_threads(TPR)) void layer_norm_kernel(const T *x, const T *__restrict__ w, const T *__restrict__ b, float eps, T *y,
+                                                                     float *__restrict__ mean_out, float *__restrict__ rstd_out, int64_t rows, int cols) {
+    using G = Group<T>;
+    constexpr int VE = G::VE, ROWS = wg_threads(TPR) / TPR;
+    __shared__ float part[2][wg_threads(TPR) / 64];
+    const int t = threadIdx.x % TPR;
+    const float per = 1.0f / (float)cols;
+    u32x4_t wv[VPT], bv[VPT];
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        const int e = (t + j * TPR) * VE;
+        wv[j] = G::load_or(w, e, cols, 1.0f);
+        bv[j] = G::load_or(b, e, cols, 0.0f);
+    }
+    for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR; row < rows; row += (int64_t)gridDim.x * ROWS) {
+        const T *xr = x + row * cols;
+        u32x4_t xv[VPT];
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            xv[j] = G::load(xr, (t + j * TPR) * VE, cols);
+        }
+        float s[1] = {0.0f};
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+#pragma unroll
+            for (int i = 0; i < VE; ++i) s[0] += G::get(xv[j], i);
+        }
+        row_sums<TPR>(s, part[0]);
+        const float mean = s[0] * per;
+        s[0] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int left = cols - (t + j * TPR) * VE;
+            keep_packed(xv[j]);
+            if (left >= VE) {
+#pragma unroll
+                for (int i = 0; i < VE; ++i) {
+                    const float d = G::get(xv[j], i) - mean;
+                    s[0] += d * d;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < VE; ++i) {
+                    const float d = G::get(xv[j], i) - mean;
+                    s[0] += i < left ? d * d : 0.0f;
+                }
+            }
+        }
+        row_sums<TPR>(s, part[1]);
+        const float rstd = 1.0f / sqrtf(s[0] * per + eps);
+        T *yr = y + row * cols;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int e = (t + j * TPR) * VE;
+            float f[VE];
+            keep_packed(xv[j]);
+            keep_packed(wv[j]);
+            keep_packed(bv[j]);
+#pragma unroll
+            for (int i = 0; i < VE; ++i) f[i] = (G::get(xv[j], i) - mean) * rstd * G::get(wv[j], i) + G::get(bv[j], i);
+            if (e < cols) G::store(yr, e, cols, G::pack(f));
+        }
+        if (t == 0) {
+            if (mean_out) mean_out[row] = mean;
+            if (rstd_out) rstd_out[row] = rstd;
+        }
+    }
+}
+
+// Backward: dx, and this workgroup's shares of dw and db.  shares [gridDim.x][2][pitch]: f32, or with one workgroup nothing, then dw and db are written here.
+template <typename T, int THREADS, int TPR, int VPT>
+__global__ __launch_bounds__(THREADS) void layer_norm_backward_kernel(const T *x, const T *dy, const T *__restrict__ w, const float *__restrict__ mean_in,
+                                                                      const float *__restrict__ rstd_in, T *dx, float *__restrict__ shares, T *__restrict__ dw,
+                                                                      T *__restrict__ db, int64_t rows, int cols, int pitch) {
+    using G = Group<T>;
+    constexpr int VE = G::VE, ROWS = THREADS / TPR;
+    static_assert(TPR <= 64 || ROWS == 1, "the waves of a row meet at the workgroup's barrier");
+    __shared__ float part[TPR > 64 ? 2 * 2 * (THREADS / 64) : 1];
+    __shared__ float added[ROWS > 1 ? ROWS / 2 * TPR * 2 * VE : 1];
+    const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+    const float per = 1.0f / (float)cols;
+    u32x4_t wv[VPT];
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        wv[j] = G::load_or(w, (t + j * TPR) * VE, cols, 1.0f);
+    }
+    float aw[VPT][VE] = {}, ab[VPT][VE] = {};
+    int turn = 0;
+    for (int64_t row = (int64_t)blockIdx.x * ROWS + sub; row < rows; row += (int64_t)gridDim.x * ROWS) {
+        u32x4_t xv[VPT], gv[VPT];
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int e = (t + j * TPR) * VE;
+            xv[j] = G::load(x + row * cols, e, cols);
+            gv[j] = G::load(dy + row * cols, e, cols);
+        }
+        const float mean = mean_in[row], rstd = rstd_in[row];
+        float s[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            keep_packed(wv[j]);
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+                // (behind the row's end dy is 0 and so is every term, or a NaN where the whole row is NaN)
+                const float d = G::get(gv[j], i), h = (G::get(xv[j], i) - mean) * rstd, g = d * G::get(wv[j], i);
+                ab[j][i] += d;
+                aw[j][i] += d * h;
+                s[0] += g;
+                s[1] += g * h;
+            }
+        }
+        if (dx) {
+            row_sums<TPR>(s, part + (TPR > 64 ? turn * 2 * (THREADS / 64) + sub * (TPR / 64) * 2 : 0));
+            turn ^= 1;
+            s[0] *= per;
+            s[1] *= per;
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                const int e = (t + j * TPR) * VE;
+                float f[VE];
+                keep_packed(xv[j]);
+                keep_packed(gv[j]);
+                keep_packed(wv[j]);
+#pragma unroll
+                for (int i = 0; i < VE; ++i) {
+                    const float d = G::get(gv[j], i), h = (G::get(xv[j], i) - mean) * rstd, g = d * G::get(wv[j], i);
+                    f[i] = rstd * (g - s[0] - h * s[1]);
+                }
+                if (e < cols) G::store(dx + row * cols, e, cols, G::pack(f));
+            }
+        }
+    }
+    if (!shares && !dw && !db) return;
+    // the rows that ran side by side: the upper half adds its sums to the lower half's, until one is left
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+#pragma unroll
+        for (int half = ROWS / 2; half; half /= 2) {
+            float *at = added + ((sub % half) * TPR + t) * 2 * VE;
+            __syncthreads();
+            if (sub >= half && sub < 2 * half)
+#pragma unroll
+                for (int i = 0; i < VE; ++i) at[i] = aw[j][i], at[VE + i] = ab[j][i];
+            __syncthreads();
+            if (sub < half)
+#pragma unroll
+                for (int i = 0; i < VE; ++i) aw[j][i] += at[i], ab[j][i] += at[VE + i];
+        }
+        const int e = (t + j * TPR) * VE;
+        if (sub != 0 || e >= cols) continue;
+        if (shares) {
+            float *mine = shares + (int64_t)blockIdx.x * 2 * pitch + e;  // pitch: whole groups
+#pragma unroll
+            for (int i = 0; i < VE; i += 4) {
+                *(f32x4_t *)(mine + i) = f32x4_t{aw[j][i], aw[j][i + 1], aw[j][i + 2], aw[j][i + 3]};
+                *(f32x4_t *)(mine + pitch + i) = f32x4_t{ab[j][i], ab[j][i + 1], ab[j][i + 2], ab[j][i + 3]};
+            }
+        } else {
+            if (dw) G::store(dw, e, cols, G::pack(aw[j]));
+            if (db) G::store(db, e, cols, G::pack(ab[j]));
+        }
+    }
+}
+
+// dw (blockIdx.y 0) and db out of n workgroups' shares: a workgroup adds 16 columns, 4 threads of 4 columns by 64 parts of the shares
+template <typename T>
+__global__ __launch_bounds__(kThreads) void add_shares_kernel(const float *__restrict__ shares, int n, int pitch, T *__restrict__ dw, T *__restrict__ db, int cols) {
+    __shared__ f32x4_t part[kThreads / 64][4];
+    const int c = threadIdx.x & 3, p = threadIdx.x >> 2;
+    const int64_t col = (int64_t)blockIdx.x * 16 + c * 4;
+    T *out = blockIdx.y ? db : dw;
+    if (!out) return;
+    f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (col < cols) {
+        const float *from = shares + blockIdx.y * (int64_t)pitch + col;
+#pragma unroll 8
+        for (int i = p; i < n; i += 64) s += *(const f32x4_t *)(from + (int64_t)i * 2 * pitch);
+    }
+#pragma unroll
+    for (int d = 4; d < 64; d *= 2)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] += __shfl_xor(s[i], d);
+    if ((threadIdx.x & 63) < 4) part[threadIdx.x >> 6][c] = s;
+    __syncthreads();
+    if (threadIdx.x >= 4 || col >= cols) return;
+    s = part[0][c];
+#pragma unroll
+    for (int i = 1; i < kThreads / 64; ++i) s += part[i][c];
+    for (int i = 0; i < 4 && col + i < cols; ++i) out[col + i] = Elem<T>::from_f32(s[i]);
+}
+
+// ---- rows longer than a workgroup's registers hold: read again for every sum, from the caches where they fit ----
+
+__device__ __forceinline__ float workgroup_sum(float v, float *part) {
+    v = lanes_sum<64>(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
     __syncthreads();
     float s = 0.0f;
-    for (int i = 0; i < kThreads / 64; ++i) s += part[i];
+    for (int i = 0; i < (int)blockDim.x / 64; ++i) s += part[i];
     return s;
 }
 
+constexpr int kLongThreads = 1024;
+
 template <typename T>
-__global__ __launch_bounds__(kThreads) void layer_norm_kernel(const T *x, const T *__restrict__ w, const T *__restrict__ b, float eps,
-                                                              T *y, float *__restrict__ mean_out, float *__restrict__ rstd_out, int64_t cols) {
-    __shared__ float part[kThreads / 64];
+__global__ __launch_bounds__(kLongThreads) void layer_norm_long_kernel(const T *x, const T *__restrict__ w, const T *__restrict__ b, float eps, T *y,
+                                                                       float *__restrict__ mean_out, float *__restrict__ rstd_out, int cols) {
+    __shared__ float part[kLongThreads / 64];
     const int64_t row = blockIdx.x;
     x += row * cols;
     y += row * cols;
+    const float per = 1.0f / (float)cols;
     float s = 0.0f;
-    for (int64_t i = threadIdx.x; i < cols; i += kThreads) s += Elem<T>::raw(x[i]);
-    const float mean = workgroup_sum(s, part) / (float)cols;
+    for (int64_t i = threadIdx.x; i < cols; i += kLongThreads) s += Elem<T>::raw(x[i]);
+    const float mean = workgroup_sum(s, part) * per;
     s = 0.0f;
-    for (int64_t i = threadIdx.x; i < cols; i += kThreads) {
+    for (int64_t i = threadIdx.x; i < cols; i += kLongThreads) {
         const float d = Elem<T>::raw(x[i]) - mean;
         s += d * d;
     }
-    const float rstd = 1.0f / sqrtf(workgroup_sum(s, part) / (float)cols + eps);
-    for (int64_t i = threadIdx.x; i < cols; i += kThreads) {
+    const float rstd = 1.0f / sqrtf(workgroup_sum(s, part) * per + eps);
+    for (int64_t i = threadIdx.x; i < cols; i += kLongThreads) {
         float v = (Elem<T>::raw(x[i]) - mean) * rstd;
         if (w) v *= Elem<T>::raw(w[i]);
         if (b) v += Elem<T>::raw(b[i]);
@@ -52,51 +357,70 @@ __global__ __launch_bounds__(kThreads) void layer_norm_kernel(const T *x, const 
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void layer_norm_backward_kernel(const T *x, const T *dy, const T *__restrict__ w,
-                                                                       const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
-                                                                       T *dx, int64_t cols) {
-    __shared__ float part[kThreads / 64];
+__global__ __launch_bounds__(kLongThreads) void layer_norm_backward_long_kernel(const T *x, const T *dy, const T *__restrict__ w, const float *__restrict__ mean_in,
+                                                                                const float *__restrict__ rstd_in, T *dx, int cols) {
+    __shared__ float part[kLongThreads / 64];
     const int64_t row = blockIdx.x;
-    const float mean = mean_in[row], rstd = rstd_in[row];
+    const float mean = mean_in[row], rstd = rstd_in[row], per = 1.0f / (float)cols;
     x += row * cols;
     dy += row * cols;
     dx += row * cols;
     float sg = 0.0f, sgh = 0.0f;
-    for (int64_t i = threadIdx.x; i < cols; i += kThreads) {
+    for (int64_t i = threadIdx.x; i < cols; i += kLongThreads) {
         const float g = Elem<T>::raw(dy[i]) * (w ? Elem<T>::raw(w[i]) : 1.0f);
         sg += g;
         sgh += g * ((Elem<T>::raw(x[i]) - mean) * rstd);
     }
-    sg = workgroup_sum(sg, part) / (float)cols;
-    sgh = workgroup_sum(sgh, part) / (float)cols;
-    for (int64_t i = threadIdx.x; i < cols; i += kThreads) {
+    sg = workgroup_sum(sg, part) * per;
+    sgh = workgroup_sum(sgh, part) * per;
+    for (int64_t i = threadIdx.x; i < cols; i += kLongThreads) {
         const float g = Elem<T>::raw(dy[i]) * (w ? Elem<T>::raw(w[i]) : 1.0f);
         dx[i] = Elem<T>::from_f32(rstd * (g - sg - (Elem<T>::raw(x[i]) - mean) * rstd * sgh));
     }
 }
 
-// one thread a column
+// one thread a column, a share for every gridDim.y-th row
 template <typename T>
-__global__ __launch_bounds__(kThreads) void layer_norm_parameters_kernel(const T *__restrict__ x, const T *__restrict__ dy, const float *__restrict__ mean,
-                                                                         const float *__restrict__ rstd, T *__restrict__ dw, T *__restrict__ db, int64_t rows,
-                                                                         int64_t cols) {
+__global__ __launch_bounds__(kThreads) void column_shares_kernel(const T *__restrict__ x, const T *__restrict__ dy, const float *__restrict__ mean,
+                                                                 const float *__restrict__ rstd, float *__restrict__ shares, int64_t rows, int cols, int pitch) {
     const int64_t col = (int64_t)blockIdx.x * kThreads + threadIdx.x;
     if (col >= cols) return;
     float sw = 0.0f, sb = 0.0f;
-    for (int64_t r = 0; r < rows; ++r) {
+#pragma unroll 4
+    for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
         const float g = Elem<T>::raw(dy[r * cols + col]);
         sb += g;
         sw += g * ((Elem<T>::raw(x[r * cols + col]) - mean[r]) * rstd[r]);
     }
-    if (dw) dw[col] = Elem<T>::from_f32(sw);
-    if (db) db[col] = Elem<T>::from_f32(sb);
+    shares[(int64_t)blockIdx.y * 2 * pitch + col] = sw;
+    shares[((int64_t)blockIdx.y * 2 + 1) * pitch + col] = sb;
 }
 
 int check_sizes(const char *name, int64_t rows, int64_t cols) {
     if (rows < 0 || cols < 1) return fail(AGH_EINVAL, "%s: %lld rows of %lld elements", name, (long long)rows, (long long)cols);
-    if (rows >= (int64_t)1 << 31 || cols >= (int64_t)1 << 31) return fail(AGH_ERANGE, "%s: %lld rows of %lld elements: too many", name, (long long)rows, (long long)cols);
+    if (rows >= (int64_t)1 << 31 || cols >= ((int64_t)1 << 31) - 65536)
+        return fail(AGH_ERANGE, "%s: %lld rows of %lld elements: too many", name, (long long)rows, (long long)cols);
     return AGH_OK;
 }
+
+template <typename T>
+struct Forward {
+    const T *x, *w, *b;
+    float eps;
+    T *y;
+    float *mean, *rstd;
+    int64_t rows;
+    int cols;
+    template <int TPR, int VPT>
+    void run() const {
+        constexpr int per_wg = wg_threads(TPR) / TPR;
+        // As many workgroups as run together, or a few times that: weight and bias are read once for several rows (a workgroup for each row: f32
+        // 16384x1001 29.4 us against 27.8, bf16 4096x16384 58 against 52), the others' loads cover what a row waits for.
+        const int64_t wgs = (rows + per_wg - 1) / per_wg, most = (int64_t)compute_units() * (TPR <= 64 || VPT > 2 ? 4 : 16);
+        hipLaunchKernelGGL((layer_norm_kernel<T, TPR, VPT>), dim3((unsigned)(wgs < most ? wgs : most)), dim3(wg_threads(TPR)), 0, stream(), x, w, b, eps, y, mean,
+                           rstd, rows, cols);
+    }
+};
 
 template <typename T>
 int forward_entry(const char *name, const void *x, const void *w, const void *b, float eps, void *y, void *mean, void *rstd, int64_t rows, int64_t cols) {
@@ -104,29 +428,101 @@ int forward_entry(const char *name, const void *x, const void *w, const void *b,
     if (!(eps >= 0.0f)) return fail(AGH_EINVAL, "%s: eps %g is negative or no number", name, (double)eps);
     if (rows == 0) return AGH_OK;
     if (!x || !y) return fail(AGH_ENULL, "%s: null input or output", name);
-    hipLaunchKernelGGL(layer_norm_kernel<T>, dim3((unsigned)rows), dim3(kThreads), 0, stream(), (const T *)x, (const T *)w, (const T *)b, eps, (T *)y,
-                       (float *)mean, (float *)rstd, cols);
+    const Forward<T> f = {(const T *)x, (const T *)w, (const T *)b, eps, (T *)y, (float *)mean, (float *)rstd, rows, (int)cols};
+    const int64_t groups = (cols + Group<T>::VE - 1) / Group<T>::VE;
+    // the fewest threads that hold the row, but a workgroup beyond 256 groups (bf16 16384x4096, 512 groups: a wave with 8 each 54.7 us, 256 threads
+    // with 2 50, 1024 threads, half of them idle, 76) and 512 threads beyond 768 (8192x8192: 256 with 4 51.1, 512 with 2 49.5, 1024 with 1 52.7)
+    if (groups <= 16) f.template run<16, 1>();
+    else if (groups <= 64) f.template run<64, 1>();
+    else if (groups <= 128) f.template run<64, 2>();
+    else if (groups <= 192) f.template run<64, 3>();
+    else if (groups <= 256) f.template run<64, 4>();
+    else if (groups <= 512) f.template run<256, 2>();
+    else if (groups <= 768) f.template run<256, 3>();
+    else if (groups <= 1024) f.template run<512, 2>();
+    else if (groups <= 1536) f.template run<512, 3>();
+    else if (groups <= 2048) f.template run<512, 4>();
+    else if (groups <= 4096) f.template run<1024, 4>();
+    else
+        hipLaunchKernelGGL(layer_norm_long_kernel<T>, dim3((unsigned)rows), dim3(kLongThreads), 0, stream(), f.x, f.w, f.b, eps, f.y, f.mean, f.rstd, f.cols);
     AGH_LAUNCH_CHECK(name);
     return AGH_OK;
 }
+
+template <typename T>
+struct Backward {
+    const char *name;
+    const T *x, *dy, *w;
+    const float *mean, *rstd;
+    T *dx, *dw, *db;
+    int64_t rows;
+    int cols, pitch;
+
+    int add(const float *shares, int64_t n) const {
+        hipLaunchKernelGGL(add_shares_kernel<T>, dim3((unsigned)((cols + 15) / 16), 2), dim3(kThreads), 0, stream(), shares, (int)n, pitch, dw, db, cols);
+        AGH_LAUNCH_CHECK(name);
+        return AGH_OK;
+    }
+    template <int THREADS, int TPR, int VPT>
+    int run() const {
+        constexpr int per_wg = THREADS / TPR;
+        // A workgroup's shares of dw and db, written and read again, cost what two to four rows do: no more workgroups than keep memory busy (bf16
+        // 16384x4096, 512 threads: 256 workgroups 98.5 us, 512 76.6, 1024 87.7; 4096x16384: 256 89.8, 512 97.7), and two turns each at least.
+        const int64_t turns = (rows + per_wg - 1) / per_wg, most = (int64_t)compute_units() * (TPR <= 64 ? 3 : VPT <= 2 ? 2 : 1);
+        int64_t wgs = (turns + 1) / 2;
+        if (wgs > most) wgs = most;
+        float *shares = nullptr;
+        if (wgs > 1 && (dw || db))
+            if (int rc = workspace((size_t)wgs * 2 * pitch * sizeof(float), (void **)&shares)) return rc;
+        hipLaunchKernelGGL((layer_norm_backward_kernel<T, THREADS, TPR, VPT>), dim3((unsigned)wgs), dim3(THREADS), 0, stream(), x, dy, w, mean, rstd, dx, shares, dw, db,
+                           rows, cols, pitch);
+        AGH_LAUNCH_CHECK(name);
+        return shares ? add(shares, wgs) : AGH_OK;
+    }
+    int run_long() const {
+        if (dw || db) {  // (before dx, which may overwrite x or dy)
+            const int64_t n = rows < 16 ? rows : rows / 16 < 64 ? rows / 16 : 64;
+            float *shares;
+            if (int rc = workspace((size_t)n * 2 * pitch * sizeof(float), (void **)&shares)) return rc;
+            hipLaunchKernelGGL(column_shares_kernel<T>, dim3((unsigned)((cols + kThreads - 1) / kThreads), (unsigned)n), dim3(kThreads), 0, stream(), x, dy, mean, rstd,
+                               shares, rows, cols, pitch);
+            AGH_LAUNCH_CHECK(name);
+            if (int rc = add(shares, n)) return rc;
+        }
+        if (dx) {
+            hipLaunchKernelGGL(layer_norm_backward_long_kernel<T>, dim3((unsigned)rows), dim3(kLongThreads), 0, stream(), x, dy, w, mean, rstd, dx, cols);
+            AGH_LAUNCH_CHECK(name);
+        }
+        return AGH_OK;
+    }
+};
 
 template <typename T>
 int backward_entry(const char *name, const void *x, const void *dy, const void *w, const void *mean, const void *rstd, void *dx, void *dw, void *db,
                    int64_t rows, int64_t cols) {
     if (int rc = check_sizes(name, rows, cols)) return rc;
     if (rows > 0 && (!x || !dy || !mean || !rstd)) return fail(AGH_ENULL, "%s: null input", name);
-    // (the parameters' gradients first: dx may overwrite x or dy)
-    if (dw || db) {
-        hipLaunchKernelGGL(layer_norm_parameters_kernel<T>, dim3((unsigned)((cols + kThreads - 1) / kThreads)), dim3(kThreads), 0, stream(), (const T *)x,
-                           (const T *)dy, (const float *)mean, (const float *)rstd, (T *)dw, (T *)db, rows, cols);
-        AGH_LAUNCH_CHECK(name);
-    }
-    if (rows > 0 && dx) {
-        hipLaunchKernelGGL(layer_norm_backward_kernel<T>, dim3((unsigned)rows), dim3(kThreads), 0, stream(), (const T *)x, (const T *)dy, (const T *)w,
-                           (const float *)mean, (const float *)rstd, (T *)dx, cols);
-        AGH_LAUNCH_CHECK(name);
-    }
-    return AGH_OK;
+    if (!dw && !db && (!dx || rows == 0)) return AGH_OK;
+    constexpr int VE = Group<T>::VE;
+    const int64_t groups = (cols + VE - 1) / VE;
+    const Backward<T> f = {name, (const T *)x, (const T *)dy, (const T *)w, (const float *)mean, (const float *)rstd, (T *)dx, (T *)dw, (T *)db, rows, (int)cols,
+                           (int)(groups * VE)};
+    if (rows == 0) return f.add(nullptr, 0);
+    // as the forward pass, but 512 threads beyond 256 groups: a thread's columns take their sums' registers too (16384x4096: bf16, 512 groups, a wave with 8 each
+    // 111 us, 256 threads with 2 79.7, 512 with 1 76.6; f32, 1024 groups, 512 with 2 145.6, 1024 with 1 147)
+    if (groups <= 16) return f.template run<256, 16, 1>();
+    if (groups <= 64) return f.template run<256, 64, 1>();
+    if (groups <= 128) return f.template run<256, 64, 2>();
+    if (groups <= 192) return f.template run<256, 64, 3>();
+    if (groups <= 256) return f.template run<256, 64, 4>();
+    if (groups <= 512) return f.template run<512, 512, 1>();
+    if (groups <= 1024) return f.template run<512, 512, 2>();
+    if (groups <= 1536) return f.template run<512, 512, 3>();
+    if (groups <= 2048) return f.template run<512, 512, 4>();
+    // (8 groups of bf16 a thread, with 128 sums, leave the compiler no registers)
+    if constexpr (VE == 4)
+        if (groups <= 4096) return f.template run<512, 512, 8>();
+    return f.run_long();
 }
 
 }  // namespace
