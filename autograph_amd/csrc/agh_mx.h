@@ -18,6 +18,11 @@ namespace mx {
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
+// 16 bytes at any element's address
+template <typename T> struct Unaligned;
+template <> struct Unaligned<float> { typedef u32x4_t vec __attribute__((aligned(4))); };
+template <> struct Unaligned<uint16_t> { typedef u32x4_t vec __attribute__((aligned(2))); };
+
 constexpr int kBlock = 32;    // values that share a scale
 constexpr int kStep = 128;    // k of a fragment
 constexpr int kFragBytes = 1024, kPieceBytes = 256;

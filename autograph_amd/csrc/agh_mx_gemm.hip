@@ -4,93 +4,75 @@
 // fed D[p][q] = sum_k P[p][k] Q[q][k] with P = b's rows and Q = a's, so that a lane's four results, p = 4 (l / 16) + r and q = l % 16, are
 // neighbours in a row of c.
 // The result is rounded once: bias and relu are applied in f32.  (agh_gemm_bf16_bias_act rounds between them, as the layers it fuses do.)
-#include "agh_mx.h"
+#include "agh_mx_direct.h"
 
 using namespace agh;
 using namespace agh::mx;
 
 namespace {
 
-typedef int i32x8_t __attribute__((ext_vector_type(8)));
-
-struct Problem {
-    const unsigned char *a, *sa, *b, *sb;  // codes and scales: a of m rows, b of n rows
-    void *c;
-    int64_t rsc, csc;  // of c, elements
-    const void *bias;  // or null
-    int64_t bias_stride;
-    int m, n, steps, act;
+// The kernels' tiles (p: columns of c, q: rows) and what a product takes in them, fitted to measured times in us: `start` + `tile` and `step` of each tile that a CU
+// takes in turn, step for 128 along k.  Measured against the estimate: 1x4096x4096 3.7 / 3.8 (16x16), 32x4096x4096 4.1 / 4.1 (16x32), 64x4096x4096
+// 5.5 / 5.4 (32x32), 512x2048x2048 6.6 / 6.6 (32x64), 1999x2047x1001 9.3 / 9.3 (128x128), 8192^3 229 / 233 (256x256).
+struct Form {
+    int bp, bq;
+    double start, tile, step;
 };
+constexpr Form kForms[] = {
+    {16, 16, 2.5, 0.2, 0.034}, {32, 16, 2.5, 0.2, 0.064}, {16, 32, 2.7, 0.2, 0.039}, {32, 32, 2.7, 0.16, 0.08}, {32, 64, 3.0, 0.5, 0.081}, {128, 128, 4.0, 1.9, 0.2125}, {256, 256, 4.0, 6.2, 0.8}};
 
-__device__ __forceinline__ i32x8_t widen(u32x4_t v) { return i32x8_t{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0}; }
-
-// both operands fp4 (format 4); S: which byte of the scale registers
-template <int SP, int SQ>
-__device__ __forceinline__ f32x4_t mfma(u32x4_t p, u32x4_t q, f32x4_t acc, uint32_t sp, uint32_t sq) {
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(p), widen(q), acc, 4, 4, SP, (int)sp, SQ, (int)sq);
-}
-
-template <typename T>
-__device__ __forceinline__ T finish(float v, float bias, int act) {
-    v += bias;
-    if (act == AGH_ACT_RELU && !(v >= 0.0f)) v = 0.0f;  // x >= 0 ? x : 0, as the Relu layer has it
-    return Elem<T>::from_f32(v);
-}
-
-// four results of a lane: columns j .. j+3 of row i
-template <typename T>
-__device__ __forceinline__ void store4(const Problem &p, f32x4_t v, int i, int j) {
-    if (i >= p.m) return;
-    T *c = (T *)p.c + i * p.rsc;
-    const T *bias = (const T *)p.bias;
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-        if (j + r < p.n) c[(j + r) * p.csc] = finish<T>(v[r], bias ? Elem<T>::raw(bias[(j + r) * p.bias_stride]) : 0.0f, p.act);
-}
-
-// Straight from memory: a wave forms 64x64 of c, a workgroup of 2x2 waves 128x128.
-template <typename T>
-__global__ __launch_bounds__(256) void mx_direct_kernel(Problem p) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int p0 = (blockIdx.x * 2 + (wave & 1)) * 64, q0 = (blockIdx.y * 2 + (wave >> 1)) * 64;
-    if (p0 >= p.n || q0 >= p.m) return;
-    const int last_p = (p.n - 1) / 16, last_q = (p.m - 1) / 16;
-    const u32x4_t *fp[4], *fq[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        fp[i] = (const u32x4_t *)(p.b + (int64_t)min(p0 / 16 + i, last_p) * p.steps * kFragBytes) + lane;
-        fq[i] = (const u32x4_t *)(p.a + (int64_t)min(q0 / 16 + i, last_q) * p.steps * kFragBytes) + lane;
+int choose_form(int64_t m, int64_t n, int64_t steps) {
+    int best = 0;
+    double least = 1e30;
+    for (int f = 0; f < (int)(sizeof(kForms) / sizeof(kForms[0])); ++f) {
+        const Form &o = kForms[f];
+        if (o.bq == 16 && m > 16) continue;
+        const double tiles = (double)((n + o.bp - 1) / o.bp) * (double)((m + o.bq - 1) / o.bq), cus = compute_units();
+        // the tiled kernels' workgroups fill a CU, one or two at a time; many small ones share it evenly
+        const double turns = o.bp >= 128 ? (double)(int64_t)((tiles + cus - 1) / cus) : tiles > cus ? tiles / cus : 1.0;
+        const double us = o.start + turns * (o.tile + o.step * (double)steps);
+        if (us < least) least = us, best = f;
     }
-    const uint32_t *sp = (const uint32_t *)(p.sb + (int64_t)(p0 / 64) * p.steps * kPieceBytes) + lane;
-    const uint32_t *sq = (const uint32_t *)(p.sa + (int64_t)(q0 / 64) * p.steps * kPieceBytes) + lane;
-    f32x4_t acc[4][4] = {};
-    for (int s = 0; s < p.steps; ++s) {
-        u32x4_t vp[4], vq[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) vp[i] = fp[i][s * 64], vq[i] = fq[i][s * 64];
-        const uint32_t xp = sp[s * 64], xq = sq[s * 64];
-#define AGH_MX_ROW(I)                                          \
-    acc[I][0] = mfma<I, 0>(vp[I], vq[0], acc[I][0], xp, xq);   \
-    acc[I][1] = mfma<I, 1>(vp[I], vq[1], acc[I][1], xp, xq);   \
-    acc[I][2] = mfma<I, 2>(vp[I], vq[2], acc[I][2], xp, xq);   \
-    acc[I][3] = mfma<I, 3>(vp[I], vq[3], acc[I][3], xp, xq);
-        AGH_MX_ROW(0) AGH_MX_ROW(1) AGH_MX_ROW(2) AGH_MX_ROW(3)
-#undef AGH_MX_ROW
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) store4<T>(p, acc[i][j], q0 + j * 16 + (lane & 15), p0 + i * 16 + (lane >> 4) * 4);
+    return best;
 }
 
 template <typename T>
-int product_launch(const char *name, const Problem &p) {
-    const int64_t gp = ((int64_t)p.n + 127) / 128, gq = ((int64_t)p.m + 127) / 128;
-    if (gq > 65535) return fail(AGH_ERANGE, "%s: %d rows: too many", name, p.m);
-    hipLaunchKernelGGL(mx_direct_kernel<T>, dim3((unsigned)gp, (unsigned)gq), dim3(256), 0, stream(), p);
-    AGH_LAUNCH_CHECK(name);
-    return AGH_OK;
-}
+struct Launch {
+    const char *name;
+    Problem p;
+    const T *x;  // a before its quantisation: null, or with 16 rows at most what the kernel quantises itself
+    int64_t rsx;
+    int k;
+
+    int grid(int form, unsigned &blocks) {
+        const Form &o = kForms[form];
+        p.tiles_p = (p.n + o.bp - 1) / o.bp;
+        p.tiles_q = (p.m + o.bq - 1) / o.bq;
+        const int64_t tiles = (int64_t)p.tiles_p * p.tiles_q;
+        if (tiles > 0x7FFFFFFFll) return fail(AGH_ERANGE, "%s: %d x %d: too many tiles", name, p.m, p.n);
+        blocks = (unsigned)tiles;
+        return AGH_OK;
+    }
+    template <bool RAW, int TP, int TQ, int WK, int U>
+    void direct(unsigned blocks) const {
+        hipLaunchKernelGGL((mx_direct_kernel<T, RAW, TP, TQ, WK, U>), dim3(blocks), dim3(WK * 64), 0, stream(), p, x, rsx, k);
+    }
+    int run(int form) {
+        unsigned blocks;
+        if (int rc = grid(form, blocks)) return rc;
+        switch (form) {
+            case 0: x ? direct<true, 1, 1, 8, 2>(blocks) : direct<false, 1, 1, 8, 4>(blocks); break;
+            case 1: x ? direct<true, 2, 1, 8, 2>(blocks) : direct<false, 2, 1, 8, 4>(blocks); break;
+            case 2: direct<false, 1, 2, 8, 4>(blocks); break;
+            case 3: direct<false, 2, 2, 4, 2>(blocks); break;
+            case 4: direct<false, 2, 4, 4, 2>(blocks); break;
+            case 5: hipLaunchKernelGGL((mx_tile_kernel<T, 128, 128, 2, 2, 4>), dim3(blocks), dim3(256), 0, stream(), p); break;
+            default: hipLaunchKernelGGL((mx_tile_kernel<T, 256, 256, 2, 4, 4>), dim3(blocks), dim3(512), 0, stream(), p); break;
+        }
+        AGH_LAUNCH_CHECK(name);
+        return AGH_OK;
+    }
+};
 
 int check_operand(const char *name, const char *what, const void *codes, const void *scales) {
     if (!codes || !scales) return fail(AGH_ENULL, "%s: null codes or scales of %s", name, what);
@@ -118,9 +100,10 @@ int gemm_entry(const char *name, int64_t m, int64_t k, int64_t n, const void *a_
         if (int rc = check_operand(name, "a", a_codes, a_scales)) return rc;
         if (int rc = check_operand(name, "b", b_codes, b_scales)) return rc;
     }
-    const Problem p = {(const unsigned char *)a_codes, (const unsigned char *)a_scales, (const unsigned char *)b_codes, (const unsigned char *)b_scales,
-                       (T *)c + off_c, rsc, csc, bias ? (const T *)bias + off_bias : nullptr, bias_stride, (int)m, (int)n, (int)steps_of(k), act};
-    return product_launch<T>(name, p);
+    const int64_t steps = steps_of(k);
+    Launch<T> l = {name, {(const unsigned char *)a_codes, (const unsigned char *)a_scales, (const unsigned char *)b_codes, (const unsigned char *)b_scales,
+                          (T *)c + off_c, rsc, csc, bias ? (const T *)bias + off_bias : nullptr, bias_stride, (int)m, (int)n, (int)steps, act, 0, 0}, nullptr, 0, 0};
+    return l.run(choose_form(m, n, steps));
 }
 
 template <typename T>
@@ -132,6 +115,14 @@ int dense_entry(const char *name, int64_t m, int64_t k, int64_t n, const void *x
     if (k > 0) {
         if (!x) return fail(AGH_ENULL, "%s: null input", name);
         if (int rc = check_operand(name, "w", w_codes, w_scales)) return rc;
+        const int64_t steps = steps_of(k);
+        const int form = choose_form(m, n, steps);
+        if (kForms[form].bq == 16 && csx == 1) {
+            // few rows: quantised by every workgroup for itself, in one launch
+            Launch<T> l = {name, {nullptr, nullptr, (const unsigned char *)w_codes, (const unsigned char *)w_scales, (T *)c + off_c, rsc, csc,
+                                  bias ? (const T *)bias + off_bias : nullptr, bias_stride, (int)m, (int)n, (int)steps, act, 0, 0}, (const T *)x + off_x, rsx, (int)k};
+            return l.run(form);
+        }
         const size_t bytes = codes_bytes(m, k);
         if (int rc = workspace(bytes + scales_bytes(m, k), &codes)) return rc;
         scales = (unsigned char *)codes + bytes;

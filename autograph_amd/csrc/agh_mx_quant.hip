@@ -3,7 +3,7 @@
 //   s = clamp(floor(log2 max |v|) - 2, -127, 127) over a block of 32, code = E2M1(v / 2^s) rounded half to even, magnitudes above 6 to 6.
 // A block with an infinity or a NaN gets the scale byte 255 and stands for 32 NaNs: E2M1 has neither, and clipping would hide them.
 // v / 2^s is a product with a power of two between 2^-125 and 2^127: exact, but where it falls below f32's smallest numbers, far below half a code.
-#include "agh_mx.h"
+#include "agh_mx_quant.h"
 
 using namespace agh;
 using namespace agh::mx;
@@ -11,39 +11,6 @@ using namespace agh::mx;
 namespace {
 
 constexpr int kThreads = 256;
-
-// a 16-byte load or store at any element's address
-template <typename T> struct Unaligned;
-template <> struct Unaligned<float> { typedef u32x4_t vec __attribute__((aligned(4))); };
-template <> struct Unaligned<uint16_t> { typedef u32x4_t vec __attribute__((aligned(2))); };
-
-__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
-
-// scale byte of a block whose largest magnitude has these bits (NaN above infinity above every number)
-__device__ __forceinline__ uint32_t scale_byte(uint32_t most) {
-    const uint32_t e = most >> 23;  // 0: zero or subnormal, below 2^-126: held to 2^-127
-    return e == 255u ? 255u : e < 2u ? 0u : e - 2u;
-}
-
-// eight values times a power of two -> eight codes
-__device__ __forceinline__ uint32_t pack8(const float *v, float by) {
-    uint32_t out = 0;
-    out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(out, v[0] * by, v[1] * by, 1.0f, 0);
-    out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(out, v[2] * by, v[3] * by, 1.0f, 1);
-    out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(out, v[4] * by, v[5] * by, 1.0f, 2);
-    out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(out, v[6] * by, v[7] * by, 1.0f, 3);
-    return out;
-}
-
-__device__ __forceinline__ void quantize_block(const float (&v)[kBlock], u32x4_t &codes, uint32_t &scale) {
-    uint32_t most = 0;
-#pragma unroll
-    for (int i = 0; i < kBlock; ++i) most = max(most, magnitude(v[i]));
-    scale = scale_byte(most);
-    const float by = scale == 255u ? 0.0f : __uint_as_float((254u - scale) << 23);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) codes[i] = scale == 255u ? 0u : pack8(v + 8 * i, by);
-}
 
 __device__ __forceinline__ int64_t code_at(int64_t row, int64_t block, int64_t steps) {
     return (((row >> 4) * steps + (block >> 2)) * 64 + (block & 3) * 16 + (row & 15)) * 16;
@@ -61,29 +28,11 @@ __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const T *__rest
     const int lane = threadIdx.x & 63;
     const int64_t rt = frag / steps;
     const int64_t row = rt * 16 + (lane & 15), block = (frag - rt * steps) * 4 + (lane >> 4), k0 = block * kBlock;
-    float v[kBlock];
-#pragma unroll
-    for (int i = 0; i < kBlock; ++i) v[i] = 0.0f;
-    if (row < rows) {
-        const T *p = x + row * rs + k0;
-        if (k0 + kBlock <= k) {
-            constexpr int VE = 16 / (int)sizeof(T);
-#pragma unroll
-            for (int i = 0; i < kBlock / VE; ++i) {
-                union { u32x4_t q; T e[VE]; } u;
-                u.q = *(const typename Unaligned<T>::vec *)(p + i * VE);
-#pragma unroll
-                for (int j = 0; j < VE; ++j) v[i * VE + j] = Elem<T>::raw(u.e[j]);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kBlock; ++i)
-                if (k0 + i < k) v[i] = Elem<T>::raw(p[i]);
-        }
-    }
+    Block<T> v;
+    v.load(x + row * rs + k0, row < rows ? (int)max((int64_t)0, k - k0) : 0);
     u32x4_t c;
     uint32_t s;
-    quantize_block(v, c, s);
+    v.quantize(c, s);
     *(u32x4_t *)(codes + frag * kFragBytes + lane * 16) = c;
     scales[scale_at(row, block, steps)] = (unsigned char)s;
 }
@@ -97,13 +46,18 @@ __global__ __launch_bounds__(kThreads) void quantize_columns_kernel(const T *__r
     if (item >= items) return;
     const int64_t rt64 = item / (steps * 4), block = item - rt64 * (steps * 4), row = rt64 * 64 + (threadIdx.x & 63), k0 = block * kBlock;
     if (row >= ((int64_t)rows + 15) / 16 * 16) return;
-    float v[kBlock];
     const T *p = x + row * rs + k0 * cs;
+    Block<T> v;
 #pragma unroll
-    for (int i = 0; i < kBlock; ++i) v[i] = row < rows && k0 + i < k ? Elem<T>::raw(p[i * cs]) : 0.0f;
+    for (int i = 0; i < Block<T>::NV; ++i) {
+        typename Block<T>::Bits u;
+#pragma unroll
+        for (int j = 0; j < Block<T>::VE; ++j) u.e[j] = row < rows && k0 + i * Block<T>::VE + j < k ? p[(i * Block<T>::VE + j) * cs] : (T)0;
+        v.v[i] = u.q;
+    }
     u32x4_t c;
     uint32_t s;
-    quantize_block(v, c, s);
+    v.quantize(c, s);
     *(u32x4_t *)(codes + code_at(row, block, steps)) = c;
     scales[scale_at(row, block, steps)] = (unsigned char)s;
 }
