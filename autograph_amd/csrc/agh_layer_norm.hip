@@ -8,13 +8,12 @@
 // groups, between its sums and its result; so the squares can be taken of deviations from the finished mean.  Up to 8 groups a lane a row belongs to
 // one wave, whose sums need neither LDS nor a barrier, longer ones to a workgroup.  Threads keep their columns from row to row: weight and bias are read
 // once, and the backward pass adds its columns' shares of dw and db in registers.
-#include "agh_internal.h"
+#include "agh_groups.h"
 
 using namespace agh;
 
 namespace {
 
-typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
@@ -55,58 +54,36 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float *part) {
     }
 }
 
-template <typename T> struct Unaligned;
-template <> struct Unaligned<float> { typedef u32x4_t vec __attribute__((aligned(4))); };
-template <> struct Unaligned<uint16_t> { typedef u32x4_t vec __attribute__((aligned(2))); };
-
-// 16 bytes of a row from element e on, at any element's address; zeros behind its end
+// A row's groups: those that pass its end behind a branch where a thread holds many (without one, each takes registers for an address of its own: bf16 4096x16384,
+// 4 groups, forward 66 us against 52), else not.
+template <typename T, bool MANY>
+__device__ __forceinline__ u32x4_t load_row(const T *row, int e, int cols) {
+    if constexpr (MANY)
+        if (e + Group<T>::VE <= cols) return *(const typename Group<T>::vec *)(row + e);
+    return Group<T>::load(row, e, cols);
+}
+// the elements of a weight that may be absent: `none` is what it stands for then
 template <typename T>
-struct Group {
-    static constexpr int VE = 16 / (int)sizeof(T);
-    typedef typename Unaligned<T>::vec vec;
-    union Bits { u32x4_t q; T e[VE]; };
-    static __device__ __forceinline__ u32x4_t load(const T *row, int e, int cols) {
-        if (e + VE <= cols) return *(const vec *)(row + e);
-        Bits b;
-        b.q = u32x4_t{0, 0, 0, 0};
+__device__ __forceinline__ u32x4_t load_or(const T *row, int e, int cols, float none) {
+    if (row) return Group<T>::load(row, e, cols);
+    float f[Group<T>::VE];
 #pragma unroll
-        for (int i = 0; i < VE; ++i)
-            if (e + i < cols) b.e[i] = row[e + i];
-        return b.q;
+    for (int i = 0; i < Group<T>::VE; ++i) f[i] = none;
+    return Group<T>::pack(f);
+}
+// with the streaming hint: forward bf16 16384x1024 15.2 -> 12.6 us, 2048x4096 8.8 -> 7.5, 16384x4096 50.4 -> 48.5
+template <typename T>
+__device__ __forceinline__ void store_group(T *row, int e, int cols, u32x4_t v) {
+    if (e + Group<T>::VE <= cols) {
+        __builtin_nontemporal_store(v, (typename Unaligned<T>::vec *)(row + e));
+        return;
     }
-    // the elements of a weight that may be absent: `none` is what it stands for then
-    static __device__ __forceinline__ u32x4_t load_or(const T *row, int e, int cols, float none) {
-        if (row) return load(row, e, cols);
-        float f[VE];
+    typename Group<T>::Bits b;
+    b.q = v;
 #pragma unroll
-        for (int i = 0; i < VE; ++i) f[i] = none;
-        return pack(f);
-    }
-    static __device__ __forceinline__ void store(T *row, int e, int cols, u32x4_t v) {
-        if (e + VE <= cols) {
-            *(vec *)(row + e) = v;
-            return;
-        }
-        Bits b;
-        b.q = v;
-#pragma unroll
-        for (int i = 0; i < VE; ++i)
-            if (e + i < cols) row[e + i] = b.e[i];
-    }
-    static __device__ __forceinline__ float get(u32x4_t v, int i) {
-        if constexpr (sizeof(T) == 4) return __uint_as_float(v[i]);
-        else return __uint_as_float(i & 1 ? v[i / 2] & 0xFFFF0000u : v[i / 2] << 16);
-    }
-    static __device__ __forceinline__ u32x4_t pack(const float (&f)[VE]) {
-        u32x4_t v;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if constexpr (sizeof(T) == 4) v[i] = __float_as_uint(f[i]);
-            else v[i] = f32x2_to_bf16x2(f[2 * i], f[2 * i + 1]);
-        }
-        return v;
-    }
-};
+    for (int i = 0; i < Group<T>::VE; ++i)
+        if (e + i < cols) row[e + i] = b.e[i];
+}
 
 // Values that stay packed: without this the compiler widens them once for all their uses, which takes a bf16 row twice the registers
 __device__ __forceinline__ void keep_packed(u32x4_t &v) {
@@ -133,15 +110,15 @@ __global__ __launch_bounds__(wg_threads(TPR)) void layer_norm_kernel(const T *x,
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
         const int e = (t + j * TPR) * VE;
-        wv[j] = G::load_or(w, e, cols, 1.0f);
-        bv[j] = G::load_or(b, e, cols, 0.0f);
+        wv[j] = load_or(w, e, cols, 1.0f);
+        bv[j] = load_or(b, e, cols, 0.0f);
     }
     for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR; row < rows; row += (int64_t)gridDim.x * ROWS) {
         const T *xr = x + row * cols;
         u32x4_t xv[VPT];
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-            xv[j] = G::load(xr, (t + j * TPR) * VE, cols);
+            xv[j] = load_row<T, (VPT > 3 && TPR > 64)>(xr, (t + j * TPR) * VE, cols);
         }
         float s[1] = {0.0f};
 #pragma unroll
@@ -182,7 +159,7 @@ __global__ __launch_bounds__(wg_threads(TPR)) void layer_norm_kernel(const T *x,
             keep_packed(bv[j]);
 #pragma unroll
             for (int i = 0; i < VE; ++i) f[i] = (G::get(xv[j], i) - mean) * rstd * G::get(wv[j], i) + G::get(bv[j], i);
-            if (e < cols) G::store(yr, e, cols, G::pack(f));
+            if (e < cols) store_group(yr, e, cols, G::pack(f));
         }
         if (t == 0) {
             if (mean_out) mean_out[row] = mean;
@@ -205,9 +182,7 @@ __global__ __launch_bounds__(THREADS) void layer_norm_backward_kernel(const T *x
     const float per = 1.0f / (float)cols;
     u32x4_t wv[VPT];
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-        wv[j] = G::load_or(w, (t + j * TPR) * VE, cols, 1.0f);
-    }
+    for (int j = 0; j < VPT; ++j) wv[j] = load_or(w, (t + j * TPR) * VE, cols, 1.0f);
     float aw[VPT][VE] = {}, ab[VPT][VE] = {};
     int turn = 0;
     for (int64_t row = (int64_t)blockIdx.x * ROWS + sub; row < rows; row += (int64_t)gridDim.x * ROWS) {
@@ -215,8 +190,8 @@ __global__ __launch_bounds__(THREADS) void layer_norm_backward_kernel(const T *x
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const int e = (t + j * TPR) * VE;
-            xv[j] = G::load(x + row * cols, e, cols);
-            gv[j] = G::load(dy + row * cols, e, cols);
+            xv[j] = load_row<T, (VPT > 3 && TPR > 64)>(x + row * cols, e, cols);
+            gv[j] = load_row<T, (VPT > 3 && TPR > 64)>(dy + row * cols, e, cols);
         }
         const float mean = mean_in[row], rstd = rstd_in[row];
         float s[2] = {0.0f, 0.0f};
@@ -236,7 +211,7 @@ __global__ __launch_bounds__(THREADS) void layer_norm_backward_kernel(const T *x
         if (dx) {
             row_sums<TPR>(s, part + (TPR > 64 ? turn * 2 * (THREADS / 64) + sub * (TPR / 64) * 2 : 0));
             turn ^= 1;
-            s[0] *= per;
+                s[0] *= per;
             s[1] *= per;
 #pragma unroll
             for (int j = 0; j < VPT; ++j) {
@@ -250,7 +225,7 @@ __global__ __launch_bounds__(THREADS) void layer_norm_backward_kernel(const T *x
                     const float d = G::get(gv[j], i), h = (G::get(xv[j], i) - mean) * rstd, g = d * G::get(wv[j], i);
                     f[i] = rstd * (g - s[0] - h * s[1]);
                 }
-                if (e < cols) G::store(dx + row * cols, e, cols, G::pack(f));
+                if (e < cols) store_group(dx + row * cols, e, cols, G::pack(f));
             }
         }
     }
@@ -280,8 +255,8 @@ __global__ __launch_bounds__(THREADS) void layer_norm_backward_kernel(const T *x
                 *(f32x4_t *)(mine + pitch + i) = f32x4_t{ab[j][i], ab[j][i + 1], ab[j][i + 2], ab[j][i + 3]};
             }
         } else {
-            if (dw) G::store(dw, e, cols, G::pack(aw[j]));
-            if (db) G::store(db, e, cols, G::pack(ab[j]));
+            if (dw) store_group(dw, e, cols, G::pack(aw[j]));
+            if (db) store_group(db, e, cols, G::pack(ab[j]));
         }
     }
 }
@@ -431,7 +406,7 @@ int forward_entry(const char *name, const void *x, const void *w, const void *b,
     const Forward<T> f = {(const T *)x, (const T *)w, (const T *)b, eps, (T *)y, (float *)mean, (float *)rstd, rows, (int)cols};
     const int64_t groups = (cols + Group<T>::VE - 1) / Group<T>::VE;
     // the fewest threads that hold the row, but a workgroup beyond 256 groups (bf16 16384x4096, 512 groups: a wave with 8 each 54.7 us, 256 threads
-    // with 2 50, 1024 threads, half of them idle, 76) and 512 threads beyond 768 (8192x8192: 256 with 4 51.1, 512 with 2 49.5, 1024 with 1 52.7)
+    // with 2 48.5, 1024 threads, half of them idle, 76) and 512 threads beyond 768 (8192x8192: 256 with 4 51.1, 512 with 2 49.5, 1024 with 1 52.7)
     if (groups <= 16) f.template run<16, 1>();
     else if (groups <= 64) f.template run<64, 1>();
     else if (groups <= 128) f.template run<64, 2>();
@@ -468,7 +443,7 @@ struct Backward {
         constexpr int per_wg = THREADS / TPR;
         // A workgroup's shares of dw and db, written and read again, cost what two to four rows do: no more workgroups than keep memory busy (bf16
         // 16384x4096, 512 threads: 256 workgroups 98.5 us, 512 76.6, 1024 87.7; 4096x16384: 256 89.8, 512 97.7), and two turns each at least.
-        const int64_t turns = (rows + per_wg - 1) / per_wg, most = (int64_t)compute_units() * (TPR <= 64 ? 3 : VPT <= 2 ? 2 : 1);
+        const int64_t turns = (rows + per_wg - 1) / per_wg, most = (int64_t)compute_units() * (TPR <= 64 ? VPT <= 2 ? 3 : 2 : VPT <= 2 ? 2 : 1);
         int64_t wgs = (turns + 1) / 2;
         if (wgs > most) wgs = most;
         float *shares = nullptr;

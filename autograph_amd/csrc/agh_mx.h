@@ -10,18 +10,13 @@
 // a byte of a register that it names itself, so the dword that lane l reads of a piece serves the four fragments of 64 rows.
 // Blocks behind k (the last 128 are always whole) hold zeros and the scale byte 0; what rows behind the last one hold is never used.
 #pragma once
-#include "agh_internal.h"
+#include "agh_groups.h"
 
 namespace agh {
 namespace mx {
 
-typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
-
-// 16 bytes at any element's address
-template <typename T> struct Unaligned;
-template <> struct Unaligned<float> { typedef u32x4_t vec __attribute__((aligned(4))); };
-template <> struct Unaligned<uint16_t> { typedef u32x4_t vec __attribute__((aligned(2))); };
 
 constexpr int kBlock = 32;    // values that share a scale
 constexpr int kStep = 128;    // k of a fragment

@@ -35,7 +35,7 @@ __global__ __launch_bounds__(WK * 64) void mx_direct_kernel(Problem g, const T *
     const uint32_t *sq = RAW ? nullptr : (const uint32_t *)(g.sa + (int64_t)(q0 / 64) * g.steps * kPieceBytes) + lane;
     const int shift_p = p0 / 16 % 4 * 8, shift_q = q0 / 16 % 4 * 8;
     const int row = q0 + (lane & 15);
-    const T *xr = RAW ? x + row * rsx + (lane >> 4) * kBlock : nullptr;
+    const T *xr = RAW ? x + (int64_t)row * rsx : nullptr;
 
     f32x4_t acc[TP][TQ];
 #pragma unroll
@@ -50,7 +50,10 @@ __global__ __launch_bounds__(WK * 64) void mx_direct_kernel(Problem g, const T *
         Block<T> raw[RAW ? count : 1];
 #pragma unroll
         for (int c = 0; c < count; ++c) {
-            if constexpr (RAW) raw[c].load(xr + (int64_t)(s + c) * kStep, row < g.m ? k - (s + c) * kStep - (lane >> 4) * kBlock : 0);
+            if constexpr (RAW) {
+                if (row < g.m) raw[c].load(xr, (s + c) * kStep + (lane >> 4) * kBlock, k);
+                else raw[c].clear();
+            }
 #pragma unroll
             for (int i = 0; i < TP; ++i) vp[c][i] = fp[i][(int64_t)(s + c) * 64];
             xp[c] = sp[(int64_t)(s + c) * 64];

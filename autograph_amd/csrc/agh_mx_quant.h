@@ -9,33 +9,23 @@ namespace mx {
 // the 16-byte groups of a block, as they were loaded
 template <typename T>
 struct Block {
-    static constexpr int VE = 16 / (int)sizeof(T), NV = kBlock / VE;
-    union Bits { u32x4_t q; T e[VE]; };
+    static constexpr int VE = Group<T>::VE, NV = kBlock / VE;
     u32x4_t v[NV];
-    // the values at p, of which `left` exist (any number: none, or more than a block), zeros behind them
-    __device__ __forceinline__ void load(const T *p, int left) {
+    // elements k0 .. of a row of k, zeros behind its end
+    __device__ __forceinline__ void load(const T *row, int k0, int k) {
+        if (k0 + kBlock <= k) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] = *(const typename Group<T>::vec *)(row + k0 + i * VE);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] = Group<T>::load(row, k0 + i * VE, k);
+        }
+    }
+    __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < NV; ++i) v[i] = u32x4_t{0, 0, 0, 0};
-        if (left <= 0) return;
-        if (left >= kBlock) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) v[i] = *(const typename Unaligned<T>::vec *)(p + i * VE);
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            Bits b;
-            b.q = u32x4_t{0, 0, 0, 0};
-#pragma unroll
-            for (int j = 0; j < VE; ++j)
-                if (i * VE + j < left) b.e[j] = p[i * VE + j];
-            v[i] = b.q;
-        }
     }
-    __device__ __forceinline__ float get(int i) const {
-        if constexpr (sizeof(T) == 4) return __uint_as_float(v[i / 4][i % 4]);
-        else return __uint_as_float(i & 1 ? v[i / 8][i % 8 / 2] & 0xFFFF0000u : v[i / 8][i % 8 / 2] << 16);
-    }
+    __device__ __forceinline__ float get(int i) const { return Group<T>::get(v[i / VE], i % VE); }
     // the bits of the largest magnitude, as f32: a NaN's are above infinity's, those above every number's
     __device__ __forceinline__ uint32_t most() const {
         if constexpr (sizeof(T) == 4) {

@@ -29,7 +29,8 @@ __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const T *__rest
     const int64_t rt = frag / steps;
     const int64_t row = rt * 16 + (lane & 15), block = (frag - rt * steps) * 4 + (lane >> 4), k0 = block * kBlock;
     Block<T> v;
-    v.load(x + row * rs + k0, row < rows ? (int)max((int64_t)0, k - k0) : 0);
+    if (row < rows) v.load(x + row * rs, (int)k0, k);
+    else v.clear();
     u32x4_t c;
     uint32_t s;
     v.quantize(c, s);
@@ -37,9 +38,46 @@ __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const T *__rest
     scales[scale_at(row, block, steps)] = (unsigned char)s;
 }
 
-// any strides, meant for rows that are neighbours in memory: a wave takes a block of 64 rows, lane l row l
+// bf16 rows that are neighbours in memory (a matrix quantised along its columns): a lane takes a block of 4 neighbouring rows, 8 bytes at every one of its 32 steps
+// along k, so a wave's load is 512 contiguous bytes.
+__global__ __launch_bounds__(kThreads) void quantize_columns_kernel(const uint16_t *__restrict__ x, int64_t cs, int rows, int k, int steps, int64_t items,
+                                                                    unsigned char *__restrict__ codes, unsigned char *__restrict__ scales) {
+    const int64_t item = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+    if (item >= items) return;
+    const int64_t group = item / (steps * 4), block = item - group * (steps * 4), row = (group * 64 + (threadIdx.x & 63)) * 4, k0 = block * kBlock;
+    if (row >= ((int64_t)rows + 15) / 16 * 16) return;
+    union Rows { u32x2_t q; uint16_t e[4]; } w[kBlock];
+    const uint16_t *p = x + row + k0 * cs;
+    if (row + 4 <= rows && k0 + kBlock <= k) {
+#pragma unroll
+        for (int i = 0; i < kBlock; ++i) w[i].q = *(const u32x2_t *)(p + i * cs);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kBlock; ++i) {
+            w[i].q = u32x2_t{0, 0};
+            if (k0 + i < k) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (row + j < rows) w[i].e[j] = p[i * cs + j];
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        Block<uint16_t> v;  // row j's values: the halves of two dwords make one
+#pragma unroll
+        for (int i = 0; i < kBlock / 2; ++i) v.v[i / 4][i % 4] = __builtin_amdgcn_perm(w[2 * i + 1].q[j / 2], w[2 * i].q[j / 2], j & 1 ? 0x07060302u : 0x05040100u);
+        u32x4_t c;
+        uint32_t s;
+        v.quantize(c, s);
+        *(u32x4_t *)(codes + code_at(row + j, block, steps)) = c;
+        scales[scale_at(row + j, block, steps)] = (unsigned char)s;
+    }
+}
+
+// any strides: a wave takes a block of 64 rows, lane l row l
 template <typename T>
-__global__ __launch_bounds__(kThreads) void quantize_columns_kernel(const T *__restrict__ x, int64_t rs, int64_t cs, int rows, int k, int steps,
+__global__ __launch_bounds__(kThreads) void quantize_strided_kernel(const T *__restrict__ x, int64_t rs, int64_t cs, int rows, int k, int steps,
                                                                     int64_t items, unsigned char *__restrict__ codes,
                                                                     unsigned char *__restrict__ scales) {
     const int64_t item = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
@@ -50,7 +88,7 @@ __global__ __launch_bounds__(kThreads) void quantize_columns_kernel(const T *__r
     Block<T> v;
 #pragma unroll
     for (int i = 0; i < Block<T>::NV; ++i) {
-        typename Block<T>::Bits u;
+        typename Group<T>::Bits u;
 #pragma unroll
         for (int j = 0; j < Block<T>::VE; ++j) u.e[j] = row < rows && k0 + i * Block<T>::VE + j < k ? p[(i * Block<T>::VE + j) * cs] : (T)0;
         v.v[i] = u.q;
@@ -66,50 +104,73 @@ __global__ __launch_bounds__(kThreads) void quantize_columns_kernel(const T *__r
 __device__ __forceinline__ float scale_value(uint32_t s) {
     return s == 255u ? __uint_as_float(0x7FC00000u) : s ? __uint_as_float(s << 23) : __uint_as_float(0x00400000u);
 }
+// codes 2 I and 2 I + 1 of a dword
+template <int I>
+__device__ __forceinline__ void decode(uint32_t c, float by, float &lo, float &hi) {
+    const auto v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, I);
+    lo = v[0] * by;
+    hi = v[1] * by;
+}
 
+// y's rows contiguous: a wave takes a fragment and writes whole rows of it, 128 values each, 16 bytes a lane.  Whole aligned groups leave with the streaming hint
+// (16384x4096 bf16 36.4 -> 26.1 us, f32 68 -> 48.7, 4096x4096 bf16 10.4 -> 8.4; unaligned ones lose by it, 16384x1001 bf16 12.8 -> 15.0).
 template <typename T>
-__global__ __launch_bounds__(kThreads) void dequantize_kernel(const unsigned char *__restrict__ codes, const unsigned char *__restrict__ scales, int rows,
-                                                              int k, int steps, int64_t items, bool by_column, T *__restrict__ y, int64_t rs, int64_t cs) {
+__global__ __launch_bounds__(kThreads) void dequantize_rows_kernel(const unsigned char *__restrict__ codes, const unsigned char *__restrict__ scales, int rows,
+                                                                   int k, int steps, int64_t frags, T *__restrict__ y, int64_t rs, bool aligned) {
+    constexpr int VE = 16 / (int)sizeof(T), LANES = kStep / VE, ROWS = 64 / LANES;  // values a lane, lanes a row, rows a store instruction
+    typedef typename std::conditional<VE == 8, uint32_t, uint16_t>::type Codes;     // of VE values
+    const int64_t frag = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+    if (frag >= frags) return;
+    const int lane = threadIdx.x & 63, at = lane % LANES * VE, block = at / kBlock;
+    const int64_t rt = frag / steps, ks = frag - rt * steps, k0 = ks * kStep + at;
+    const unsigned char *from = codes + frag * kFragBytes + block * 256 + at % kBlock / 2;
+    uint32_t c[16 / ROWS], s[16 / ROWS];
+#pragma unroll
+    for (int i = 0; i < 16 / ROWS; ++i) {
+        const int r = i * ROWS + lane / LANES;
+        c[i] = *(const Codes *)(from + r * 16);
+        s[i] = rt * 16 + r < rows ? scales[scale_at(rt * 16 + r, ks * 4 + block, steps)] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < 16 / ROWS; ++i) {
+        const int64_t row = rt * 16 + i * ROWS + lane / LANES;
+        const float by = scale_value(s[i]);
+        float f[8];
+        decode<0>(c[i], by, f[0], f[1]);
+        decode<1>(c[i], by, f[2], f[3]);
+        if constexpr (VE == 8) decode<2>(c[i], by, f[4], f[5]), decode<3>(c[i], by, f[6], f[7]);
+        union { u32x4_t q; T e[VE]; } u;
+#pragma unroll
+        for (int j = 0; j < VE; ++j) u.e[j] = Elem<T>::from_f32(f[j]);
+        if (row >= rows || k0 >= k) continue;
+        T *to = y + row * rs + k0;
+        if (aligned && k0 + VE <= k) __builtin_nontemporal_store(u.q, (u32x4_t *)to);
+        else if (k0 + VE <= k) *(typename Unaligned<T>::vec *)to = u.q;
+        else
+#pragma unroll
+            for (int j = 0; j < VE; ++j)
+                if (k0 + j < k) to[j] = u.e[j];
+    }
+}
+
+// any strides: a wave takes a block of 64 rows, lane l row l
+template <typename T>
+__global__ __launch_bounds__(kThreads) void dequantize_strided_kernel(const unsigned char *__restrict__ codes, const unsigned char *__restrict__ scales, int rows,
+                                                                      int k, int steps, int64_t items, T *__restrict__ y, int64_t rs, int64_t cs) {
     const int64_t item = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
     if (item >= items) return;
-    const int lane = threadIdx.x & 63;
-    int64_t row, block;
-    if (by_column) {
-        const int64_t rt64 = item / (steps * 4);
-        row = rt64 * 64 + lane;
-        block = item - rt64 * (steps * 4);
-    } else {
-        const int64_t rt = item / steps;
-        row = rt * 16 + (lane & 15);
-        block = (item - rt * steps) * 4 + (lane >> 4);
-    }
-    const int64_t k0 = block * kBlock;
+    const int64_t rt64 = item / (steps * 4), block = item - rt64 * (steps * 4), row = rt64 * 64 + (threadIdx.x & 63), k0 = block * kBlock;
     if (row >= rows || k0 >= k) return;
     const u32x4_t c = *(const u32x4_t *)(codes + code_at(row, block, steps));
     const float by = scale_value(scales[scale_at(row, block, steps)]);
-    float v[kBlock];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const auto p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[i], 1.0f, 0), p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[i], 1.0f, 1);
-        const auto p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[i], 1.0f, 2), p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[i], 1.0f, 3);
-        v[8 * i] = p0[0], v[8 * i + 1] = p0[1], v[8 * i + 2] = p1[0], v[8 * i + 3] = p1[1];
-        v[8 * i + 4] = p2[0], v[8 * i + 5] = p2[1], v[8 * i + 6] = p3[0], v[8 * i + 7] = p3[1];
-    }
     T *p = y + row * rs + k0 * cs;
-    if (cs == 1 && k0 + kBlock <= k) {
-        constexpr int VE = 16 / (int)sizeof(T);
-#pragma unroll
-        for (int i = 0; i < kBlock / VE; ++i) {
-            union { u32x4_t q; T e[VE]; } u;
-#pragma unroll
-            for (int j = 0; j < VE; ++j) u.e[j] = Elem<T>::from_f32(v[i * VE + j] * by);
-            *(typename Unaligned<T>::vec *)(p + i * VE) = u.q;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < kBlock; ++i)
-            if (k0 + i < k) p[i * cs] = Elem<T>::from_f32(v[i] * by);
-    }
+    agh::gemm::static_for<kBlock / 2>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        float lo, hi;
+        decode<i % 4>(c[i / 4], by, lo, hi);
+        if (k0 + 2 * i < k) p[2 * i * cs] = Elem<T>::from_f32(lo);
+        if (k0 + 2 * i + 1 < k) p[(2 * i + 1) * cs] = Elem<T>::from_f32(hi);
+    });
 }
 
 int check_sizes(const char *name, int64_t rows, int64_t k) {
@@ -146,12 +207,16 @@ int dequantize_entry(const char *name, const void *codes, const void *scales, in
     if ((rows > 1 && rs == 0) || (k > 1 && cs == 0)) return fail(AGH_EINVAL, "%s: the elements of y must be distinct addresses", name);
     if (int rc = check_quantized(name, codes, scales)) return rc;
     const int steps = (int)steps_of(k);
-    const bool by_column = (rs < 0 ? -rs : rs) < (cs < 0 ? -cs : cs);
-    const int64_t items = by_column ? (rows + 63) / 64 * steps * 4 : (rows + 15) / 16 * steps;
+    const unsigned char *c = (const unsigned char *)codes, *s = (const unsigned char *)scales;
+    T *to = (T *)y + off;
+    const int64_t items = cs == 1 ? (rows + 15) / 16 * steps : (rows + 63) / 64 * steps * 4;
     unsigned blocks;
     if (int rc = waves_grid(name, items, blocks)) return rc;
-    hipLaunchKernelGGL(dequantize_kernel<T>, dim3(blocks), dim3(kThreads), 0, stream(), (const unsigned char *)codes, (const unsigned char *)scales,
-                       (int)rows, (int)k, steps, items, by_column, (T *)y + off, rs, cs);
+    if (cs == 1)
+        hipLaunchKernelGGL(dequantize_rows_kernel<T>, dim3(blocks), dim3(kThreads), 0, stream(), c, s, (int)rows, (int)k, steps, items, to, rs,
+                           ((uintptr_t)to & 15) == 0 && rs * (int64_t)sizeof(T) % 16 == 0);
+    else
+        hipLaunchKernelGGL(dequantize_strided_kernel<T>, dim3(blocks), dim3(kThreads), 0, stream(), c, s, (int)rows, (int)k, steps, items, to, rs, cs);
     AGH_LAUNCH_CHECK(name);
     return AGH_OK;
 }
@@ -170,10 +235,25 @@ int quantize_launch(const char *name, const T *x, int64_t rs, int64_t cs, int64_
         if (int rc = waves_grid(name, frags, blocks)) return rc;
         hipLaunchKernelGGL(quantize_rows_kernel<T>, dim3(blocks), dim3(kThreads), 0, stream(), x, rs, (int)rows, (int)k, steps, frags,
                            (unsigned char *)codes, (unsigned char *)scales);
-    } else {
+        AGH_LAUNCH_CHECK(name);
+        return AGH_OK;
+    }
+    // Four rows a lane for whole 8-byte groups and as many waves as there are SIMDs twice over (bf16 by columns, us, against one row a lane: 16384x4096 38.7 / 49.9,
+    // 4096x4096 11.1 / 12.8; but 2048x1000, 256 waves, 9.5 / 5.7, 16384x1001 19.1 / 13.6; f32 gains nothing: 69.6 / 66.6).
+    if constexpr (sizeof(T) == 2) {
+        const int64_t items = (rows + 255) / 256 * steps * 4;
+        if (rs == 1 && cs % 4 == 0 && ((uintptr_t)x & 7) == 0 && items >= 8ll * compute_units()) {
+            if (int rc = waves_grid(name, items, blocks)) return rc;
+            hipLaunchKernelGGL(quantize_columns_kernel, dim3(blocks), dim3(kThreads), 0, stream(), x, cs, (int)rows, (int)k, steps, items, (unsigned char *)codes,
+                               (unsigned char *)scales);
+            AGH_LAUNCH_CHECK(name);
+            return AGH_OK;
+        }
+    }
+    {
         const int64_t items = (rows + 63) / 64 * steps * 4;
         if (int rc = waves_grid(name, items, blocks)) return rc;
-        hipLaunchKernelGGL(quantize_columns_kernel<T>, dim3(blocks), dim3(kThreads), 0, stream(), x, rs, cs, (int)rows, (int)k, steps, items,
+        hipLaunchKernelGGL(quantize_strided_kernel<T>, dim3(blocks), dim3(kThreads), 0, stream(), x, rs, cs, (int)rows, (int)k, steps, items,
                            (unsigned char *)codes, (unsigned char *)scales);
     }
     AGH_LAUNCH_CHECK(name);

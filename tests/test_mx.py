@@ -139,7 +139,7 @@ def test_the_oracle():
 
 # ---- on the GPU ----
 
-SHAPES = [(1, 1), (1, 32), (3, 31), (16, 128), (17, 129), (64, 127), (65, 64), (5, 1001), (130, 300), (200, 33)]
+SHAPES = [(1, 1), (1, 32), (3, 31), (16, 128), (17, 129), (64, 127), (65, 64), (5, 1001), (130, 300), (200, 33), (257, 259), (33, 530), (128, 256)]
 
 
 @gpu
@@ -182,6 +182,27 @@ def test_quantize_borders(ag, dtype):
         want = mxfp4.quantize(ref)
         assert np.array_equal(got[1], want[1])
         assert np.array_equal(got[0], want[0])
+
+
+@gpu
+def test_dequantize_every_code_and_scale(ag):
+    """All codes under all scale bytes, by rows, by columns and into a strided matrix: exact in both types, subnormal values too."""
+    codes = np.tile(np.arange(16, dtype=np.uint8), (256, 6))[:, :90]
+    scales = np.repeat(np.arange(256, dtype=np.uint8)[:, None], 3, 1)
+    want = mxfp4.values(codes, scales)
+    want = np.where(np.abs(want) >= 2.0**128, np.copysign(np.inf, want), want)
+    for q, ref in ((ag.MxTensor.from_arrays(codes, scales), want), (ag.MxTensor.from_arrays(codes.T, scales.T, axis=0), want.T)):
+        for dtype in ("f32", "bf16"):
+            assert np.array_equal(values_of(q.dequantize(dtype)), ref, equal_nan=True)
+            assert np.array_equal(values_of(q.t().dequantize(dtype)), ref.T, equal_nan=True)
+    wide = ag.Tensor.zeros((256 * 2, 90 * 3), "f32")
+    q = ag.MxTensor.from_arrays(codes, scales)
+    ag._ffi.check(ag.lib.agh_dequantize_mxfp4_f32(q.codes.ptr, q.scales.ptr, 256, 90, wide._ptr(), 5, 2 * 270, 3))
+    got = wide.into_array().ravel()
+    at = 5 + np.arange(256)[:, None] * 540 + np.arange(90)[None, :] * 3
+    assert np.array_equal(got[at].astype(np.float64), want, equal_nan=True)
+    got[at] = 0
+    assert not got.any()
 
 
 @gpu
