@@ -37,6 +37,9 @@ int choose_form(int64_t m, int64_t n, int64_t steps) {
 }
 
 template <typename T>
+bool rows_aligned(const T *c, int64_t rs) { return ((uintptr_t)c & 15) == 0 && rs * (int64_t)sizeof(T) % 16 == 0; }
+
+template <typename T>
 struct Launch {
     const char *name;
     Problem p;
@@ -67,7 +70,7 @@ struct Launch {
             case 3: direct<false, 2, 2, 4, 2>(blocks); break;
             case 4: direct<false, 2, 4, 4, 2>(blocks); break;
             case 5: hipLaunchKernelGGL((mx_tile_kernel<T, 128, 128, 2, 2, 4>), dim3(blocks), dim3(256), 0, stream(), p); break;
-            default: hipLaunchKernelGGL((mx_tile_kernel<T, 256, 256, 2, 4, 4>), dim3(blocks), dim3(512), 0, stream(), p); break;
+            default: hipLaunchKernelGGL((mx_tile_kernel<T, 256, 256, 4, 2, 4>), dim3(blocks), dim3(512), 0, stream(), p); break;
         }
         AGH_LAUNCH_CHECK(name);
         return AGH_OK;
@@ -102,7 +105,7 @@ int gemm_entry(const char *name, int64_t m, int64_t k, int64_t n, const void *a_
     }
     const int64_t steps = steps_of(k);
     Launch<T> l = {name, {(const unsigned char *)a_codes, (const unsigned char *)a_scales, (const unsigned char *)b_codes, (const unsigned char *)b_scales,
-                          (T *)c + off_c, rsc, csc, bias ? (const T *)bias + off_bias : nullptr, bias_stride, (int)m, (int)n, (int)steps, act, 0, 0}, nullptr, 0, 0};
+                          (T *)c + off_c, rsc, csc, bias ? (const T *)bias + off_bias : nullptr, bias_stride, (int)m, (int)n, (int)steps, act, rows_aligned<T>((T *)c + off_c, rsc), 0, 0}, nullptr, 0, 0};
     return l.run(choose_form(m, n, steps));
 }
 
@@ -120,7 +123,7 @@ int dense_entry(const char *name, int64_t m, int64_t k, int64_t n, const void *x
         if (kForms[form].bq == 16 && csx == 1) {
             // few rows: quantised by every workgroup for itself, in one launch
             Launch<T> l = {name, {nullptr, nullptr, (const unsigned char *)w_codes, (const unsigned char *)w_scales, (T *)c + off_c, rsc, csc,
-                                  bias ? (const T *)bias + off_bias : nullptr, bias_stride, (int)m, (int)n, (int)steps, act, 0, 0}, (const T *)x + off_x, rsx, (int)k};
+                                  bias ? (const T *)bias + off_bias : nullptr, bias_stride, (int)m, (int)n, (int)steps, act, false, 0, 0}, (const T *)x + off_x, rsx, (int)k};
             return l.run(form);
         }
         const size_t bytes = codes_bytes(m, k);

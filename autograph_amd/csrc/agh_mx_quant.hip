@@ -38,41 +38,41 @@ __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const T *__rest
     scales[scale_at(row, block, steps)] = (unsigned char)s;
 }
 
-// bf16 rows that are neighbours in memory (a matrix quantised along its columns): a lane takes a block of 4 neighbouring rows, 8 bytes at every one of its 32 steps
-// along k, so a wave's load is 512 contiguous bytes.
-__global__ __launch_bounds__(kThreads) void quantize_columns_kernel(const uint16_t *__restrict__ x, int64_t cs, int rows, int k, int steps, int64_t items,
+// bf16 rows that are neighbours in memory (a matrix quantised along its columns): a workgroup takes 64 rows x 128 k, whose 128 pieces of memory, 64 values each, it
+// copies to LDS in 16-byte groups.  A wave then reads a fragment of it with the reads that transpose: within 16 lanes, lanes 4 j .. 4 j + 3 name the 16 rows of k + j, and
+// lane i receives row i's values of k .. k + 3; so lane l ends with the block l / 16 of row l % 16.
+constexpr int kTilePitch = 160;  // bytes of 64 rows at one k: four neighbouring k lie in different banks
+__global__ __launch_bounds__(kThreads) void quantize_columns_kernel(const uint16_t *__restrict__ x, int64_t cs, int rows, int k, int steps,
                                                                     unsigned char *__restrict__ codes, unsigned char *__restrict__ scales) {
-    const int64_t item = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
-    if (item >= items) return;
-    const int64_t group = item / (steps * 4), block = item - group * (steps * 4), row = (group * 64 + (threadIdx.x & 63)) * 4, k0 = block * kBlock;
-    if (row >= ((int64_t)rows + 15) / 16 * 16) return;
-    union Rows { u32x2_t q; uint16_t e[4]; } w[kBlock];
-    const uint16_t *p = x + row + k0 * cs;
-    if (row + 4 <= rows && k0 + kBlock <= k) {
+    __shared__ __align__(16) unsigned char tile[kStep * kTilePitch];
+    // (neighbouring workgroups take neighbouring rows: what they read together are whole rows of memory)
+    const int64_t groups = ((int64_t)rows + 63) / 64, ks = blockIdx.x / groups, rt64 = blockIdx.x - ks * groups;
+    const int row0 = (int)rt64 * 64, k0 = (int)ks * kStep, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-        for (int i = 0; i < kBlock; ++i) w[i].q = *(const u32x2_t *)(p + i * cs);
-    } else {
-#pragma unroll
-        for (int i = 0; i < kBlock; ++i) {
-            w[i].q = u32x2_t{0, 0};
-            if (k0 + i < k) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (row + j < rows) w[i].e[j] = p[i * cs + j];
-            }
-        }
+    for (int i = 0; i < 4; ++i) {
+        const int kk = i * 32 + (threadIdx.x >> 3), e = (threadIdx.x & 7) * 8;
+        u32x4_t v = {0, 0, 0, 0};
+        if (k0 + kk < k) v = Group<uint16_t>::load(x + (int64_t)(k0 + kk) * cs, row0 + e, rows);
+        *(u32x4_t *)(tile + kk * kTilePitch + e * 2) = v;
     }
+    __syncthreads();
+    const int row = row0 + wave * 16 + (lane & 15);
+    if (row0 + wave * 16 >= rows) return;
+    typedef short s16x4_t __attribute__((ext_vector_type(4)));
+    Block<uint16_t> v;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        Block<uint16_t> v;  // row j's values: the halves of two dwords make one
-#pragma unroll
-        for (int i = 0; i < kBlock / 2; ++i) v.v[i / 4][i % 4] = __builtin_amdgcn_perm(w[2 * i + 1].q[j / 2], w[2 * i].q[j / 2], j & 1 ? 0x07060302u : 0x05040100u);
-        u32x4_t c;
-        uint32_t s;
-        v.quantize(c, s);
-        *(u32x4_t *)(codes + code_at(row + j, block, steps)) = c;
-        scales[scale_at(row + j, block, steps)] = (unsigned char)s;
+    for (int i = 0; i < 8; ++i) {
+        const unsigned char *at = tile + ((lane >> 4) * kBlock + i * 4 + (lane & 15) / 4) * kTilePitch + wave * 32 + (lane & 3) * 8;
+        const s16x4_t r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t *)at);
+        const u32x2_t q = __builtin_bit_cast(u32x2_t, r);
+        v.v[i / 2][i % 2 * 2] = q[0];
+        v.v[i / 2][i % 2 * 2 + 1] = q[1];
     }
+    u32x4_t c;
+    uint32_t s;
+    v.quantize(c, s);
+    *(u32x4_t *)(codes + (((rt64 * 4 + wave) * steps + ks) * 64 + lane) * 16) = c;
+    scales[scale_at(row, ks * 4 + (lane >> 4), steps)] = (unsigned char)s;
 }
 
 // any strides: a wave takes a block of 64 rows, lane l row l
@@ -238,13 +238,11 @@ int quantize_launch(const char *name, const T *x, int64_t rs, int64_t cs, int64_
         AGH_LAUNCH_CHECK(name);
         return AGH_OK;
     }
-    // Four rows a lane for whole 8-byte groups and as many waves as there are SIMDs twice over (bf16 by columns, us, against one row a lane: 16384x4096 38.7 / 49.9,
-    // 4096x4096 11.1 / 12.8; but 2048x1000, 256 waves, 9.5 / 5.7, 16384x1001 19.1 / 13.6; f32 gains nothing: 69.6 / 66.6).
     if constexpr (sizeof(T) == 2) {
-        const int64_t items = (rows + 255) / 256 * steps * 4;
-        if (rs == 1 && cs % 4 == 0 && ((uintptr_t)x & 7) == 0 && items >= 8ll * compute_units()) {
-            if (int rc = waves_grid(name, items, blocks)) return rc;
-            hipLaunchKernelGGL(quantize_columns_kernel, dim3(blocks), dim3(kThreads), 0, stream(), x, cs, (int)rows, (int)k, steps, items, (unsigned char *)codes,
+        if (rs == 1 && rows >= 16) {
+            const int64_t tiles = (rows + 63) / 64 * steps;
+            if (tiles > 0x7FFFFFFFll) return fail(AGH_ERANGE, "%s: too many blocks", name);
+            hipLaunchKernelGGL(quantize_columns_kernel, dim3((unsigned)tiles), dim3(kThreads), 0, stream(), x, cs, (int)rows, (int)k, steps, (unsigned char *)codes,
                                (unsigned char *)scales);
             AGH_LAUNCH_CHECK(name);
             return AGH_OK;
