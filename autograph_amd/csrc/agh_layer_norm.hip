@@ -444,7 +444,7 @@ struct Backward {
         // A workgroup's shares of dw and db, written and read again, cost what two to four rows do: no more workgroups than keep memory busy (bf16
         // 16384x4096, 512 threads: 256 workgroups 98.5 us, 512 76.6, 1024 87.7; 4096x16384: 256 89.8, 512 97.7), and two turns each at least.
         const int64_t turns = (rows + per_wg - 1) / per_wg, most = (int64_t)compute_units() * (TPR <= 64 ? VPT <= 2 ? 3 : 2 : VPT <= 2 ? 2 : 1);
-        int64_t wgs = (turns + 1) / 2;
+        int64_t wgs = THREADS == 1024 ? 1 : (turns + 1) / 2;
         if (wgs > most) wgs = most;
         float *shares = nullptr;
         if (wgs > 1 && (dw || db))
@@ -485,6 +485,10 @@ int backward_entry(const char *name, const void *x, const void *dy, const void *
     if (rows == 0) return f.add(nullptr, 0);
     // as the forward pass, but 512 threads beyond 256 groups: a thread's columns take their sums' registers too (16384x4096: bf16, 512 groups, a wave with 8 each
     // 111 us, 256 threads with 2 79.7, 512 with 1 76.6; f32, 1024 groups, 512 with 2 145.6, 1024 with 1 147)
+    // short rows and few turns of 1024 threads: one workgroup, which needs no second launch (f32, us against two: 100x84 7.8 / 11.7, 128x84 9.4 / 10.3, 256x60 5.9 / 10.3; 256x84
+    // 16.2 / 10.3, 512x60 9.1 / 8.3)
+    if (groups <= 16 && rows <= 256) return f.template run<1024, 16, 1>();
+    if (groups <= 64 && rows <= 128) return f.template run<1024, 64, 1>();
     if (groups <= 16) return f.template run<256, 16, 1>();
     if (groups <= 64) return f.template run<256, 64, 1>();
     if (groups <= 128) return f.template run<256, 64, 2>();

@@ -3,7 +3,7 @@
 // in the waves' order.  With few rows of a (one token, a handful of requests) this is a pass over b at the speed of memory.
 //
 // RAW: a is not quantised yet.  A lane quantises what its place in the fragment holds, 32 neighbours of one row, so the values never leave its
-// registers; every workgroup does it again, which for 16 rows is less than a launch of its own.
+// registers; every workgroup does it again, which for few rows is less than a launch of its own.
 #pragma once
 #include "agh_mx_quant.h"
 #include "agh_mx_tile.h"
@@ -13,7 +13,7 @@ namespace mx {
 
 template <typename T, bool RAW, int TP, int TQ, int WK, int U>
 __global__ __launch_bounds__(WK * 64) void mx_direct_kernel(Problem g, const T *__restrict__ x, int64_t rsx, int k) {
-    static_assert((TP == 1 || TP == 2 || TP == 4) && (TQ == 1 || TQ == 2 || TQ == 4) && (!RAW || TQ == 1), "a tile's rows lie in one piece of the scales");
+    static_assert((TP == 1 || TP == 2 || TP == 4) && (TQ == 1 || TQ == 2 || TQ == 4), "a tile's rows lie in one piece of the scales");
     __shared__ f32x4_t sums[WK][TP * TQ][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // a run of tiles for every XCD (workgroup id mod 8), p fastest: neighbours share pieces of scales, and a
@@ -34,8 +34,7 @@ __global__ __launch_bounds__(WK * 64) void mx_direct_kernel(Problem g, const T *
     const uint32_t *sp = (const uint32_t *)(g.sb + (int64_t)(p0 / 64) * g.steps * kPieceBytes) + lane;
     const uint32_t *sq = RAW ? nullptr : (const uint32_t *)(g.sa + (int64_t)(q0 / 64) * g.steps * kPieceBytes) + lane;
     const int shift_p = p0 / 16 % 4 * 8, shift_q = q0 / 16 % 4 * 8;
-    const int row = q0 + (lane & 15);
-    const T *xr = RAW ? x + (int64_t)row * rsx : nullptr;
+    const int row = q0 + (lane & 15);  // (RAW) of the first fragment of a
 
     f32x4_t acc[TP][TQ];
 #pragma unroll
@@ -47,12 +46,15 @@ __global__ __launch_bounds__(WK * 64) void mx_direct_kernel(Problem g, const T *
         constexpr int count = decltype(countc)::value;
         u32x4_t vp[count][TP], vq[count][TQ];
         uint32_t xp[count], xq[count];
-        Block<T> raw[RAW ? count : 1];
+        Block<T> raw[RAW ? count : 1][TQ];
 #pragma unroll
         for (int c = 0; c < count; ++c) {
             if constexpr (RAW) {
-                if (row < g.m) raw[c].load(xr, (s + c) * kStep + (lane >> 4) * kBlock, k);
-                else raw[c].clear();
+#pragma unroll
+                for (int j = 0; j < TQ; ++j) {
+                    if (row + 16 * j < g.m) raw[c][j].load(x + (int64_t)(row + 16 * j) * rsx, (s + c) * kStep + (lane >> 4) * kBlock, k);
+                    else raw[c][j].clear();
+                }
             }
 #pragma unroll
             for (int i = 0; i < TP; ++i) vp[c][i] = fp[i][(int64_t)(s + c) * 64];
@@ -65,8 +67,17 @@ __global__ __launch_bounds__(WK * 64) void mx_direct_kernel(Problem g, const T *
         }
 #pragma unroll
         for (int c = 0; c < count; ++c) {
-            if constexpr (RAW) raw[c].quantize(vq[c][0], xq[c]);
-            else xq[c] >>= shift_q;
+            if constexpr (RAW) {
+                xq[c] = 0;
+#pragma unroll
+                for (int j = 0; j < TQ; ++j) {
+                    uint32_t scale;
+                    raw[c][j].quantize(vq[c][j], scale);
+                    xq[c] |= scale << (8 * j);
+                }
+            } else {
+                xq[c] >>= shift_q;
+            }
             xp[c] >>= shift_p;
             agh::gemm::static_for<TP>([&](auto ic) {
                 agh::gemm::static_for<TQ>([&](auto jc) {

@@ -11,15 +11,17 @@ using namespace agh::mx;
 
 namespace {
 
-// The kernels' tiles (p: columns of c, q: rows) and what a product takes in them, fitted to measured times in us: `start` + `tile` and `step` of each tile that a CU
-// takes in turn, step for 128 along k.  Measured against the estimate: 1x4096x4096 3.7 / 3.8 (16x16), 32x4096x4096 4.1 / 4.1 (16x32), 64x4096x4096
-// 5.5 / 5.4 (32x32), 512x2048x2048 6.6 / 6.6 (32x64), 1999x2047x1001 9.3 / 9.3 (128x128), 8192^3 229 / 233 (256x256).
+// The kernels' tiles (p: columns of c, q: rows) and what a product takes in them, fitted to measured times in us: `start`, and for each tile that a CU takes in turn
+// `tile` + `step` for every 128 of k, but at least `least` (fetching the kernel's code, storing the result).  Measured against the estimate: 1x4096x4096 3.7 /
+// 3.8 (16x16), 32x4096x4096 4.1 / 4.1 (16x32), 64x4096x4096 5.5 / 5.4 (32x32), 512x2048x2048 6.5 / 6.9 (32x64), 1024x4096x1024 7.9 / 7.8 (64x64),
+// 1999x2047x1001 9.3 / 9.3 (128x128), 16384x4096x4096 125 / 116 (256x256).  Over 220 products of sizes drawn at random the form chosen takes 1.02 of the best one's time in
+// the mean.  (128x128 tiles with k split between two halves of a workgroup took 11.5 instead of 12.4 us at 2048x4096x1000 and lost where k is short; not taken.)
 struct Form {
     int bp, bq;
-    double start, tile, step;
+    double start, tile, step, least;
 };
-constexpr Form kForms[] = {
-    {16, 16, 2.5, 0.2, 0.034}, {32, 16, 2.5, 0.2, 0.064}, {16, 32, 2.7, 0.2, 0.039}, {32, 32, 2.7, 0.16, 0.08}, {32, 64, 3.0, 0.5, 0.081}, {128, 128, 4.0, 1.9, 0.2125}, {256, 256, 4.0, 6.2, 0.8}};
+constexpr Form kForms[] = {{16, 16, 2.5, 0.2, 0.034, 0.4},  {32, 16, 2.5, 0.2, 0.064, 0.5}, {16, 32, 2.7, 0.2, 0.039, 0.62},   {32, 32, 2.7, 0.16, 0.08, 0.6},
+                           {32, 64, 3.0, 0.7, 0.075, 1.25}, {64, 64, 3.2, 2.0, 0.08, 2.7},  {128, 128, 4.0, 1.9, 0.2125, 0.0}, {256, 256, 4.0, 6.2, 0.68, 0.0}};
 
 int choose_form(int64_t m, int64_t n, int64_t steps) {
     int best = 0;
@@ -30,10 +32,19 @@ int choose_form(int64_t m, int64_t n, int64_t steps) {
         const double tiles = (double)((n + o.bp - 1) / o.bp) * (double)((m + o.bq - 1) / o.bq), cus = compute_units();
         // the tiled kernels' workgroups fill a CU, one or two at a time; many small ones share it evenly
         const double turns = o.bp >= 128 ? (double)(int64_t)((tiles + cus - 1) / cus) : tiles > cus ? tiles / cus : 1.0;
-        const double us = o.start + turns * (o.tile + o.step * (double)steps);
+        const double each = o.tile + o.step * (double)steps, us = o.start + turns * (each > o.least ? each : o.least);
         if (us < least) least = us, best = f;
     }
     return best;
+}
+
+// Whether Dense's input is quantised in the product's launch, by every workgroup again, instead of by a launch of its own (2.5 to 2.9 us, and as much of the host's time):
+// up to 16 rows always (1x4096x4096 4.6 us against 3.7 + 2.5, 16x4096x4096 6.6 against 3.7 + 2.5), to about 500 where no CU has a second tile and k is short (64x256x256 3.5
+// against 2.8 + 2.9, 100x1000x300 4.8 against 2.8 + 2.8; 200x2000x100 6.8 against 3.0 + 2.8, 64x4096x4096 11.3 against 5.4 + 2.7).
+bool quantises_itself(int form, int64_t m, int64_t n, int64_t steps) {
+    const Form &o = kForms[form];
+    if (o.bq == 16) return true;
+    return o.bq == 32 && steps <= 8 && (m + o.bq - 1) / o.bq * ((n + o.bp - 1) / o.bp) <= compute_units();
 }
 
 template <typename T>
@@ -43,7 +54,7 @@ template <typename T>
 struct Launch {
     const char *name;
     Problem p;
-    const T *x;  // a before its quantisation: null, or with 16 rows at most what the kernel quantises itself
+    const T *x;  // null, or a before its quantisation, which the kernel does itself
     int64_t rsx;
     int k;
 
@@ -66,10 +77,11 @@ struct Launch {
         switch (form) {
             case 0: x ? direct<true, 1, 1, 8, 2>(blocks) : direct<false, 1, 1, 8, 4>(blocks); break;
             case 1: x ? direct<true, 2, 1, 8, 2>(blocks) : direct<false, 2, 1, 8, 4>(blocks); break;
-            case 2: direct<false, 1, 2, 8, 4>(blocks); break;
-            case 3: direct<false, 2, 2, 4, 2>(blocks); break;
+            case 2: x ? direct<true, 1, 2, 8, 1>(blocks) : direct<false, 1, 2, 8, 4>(blocks); break;
+            case 3: x ? direct<true, 2, 2, 4, 1>(blocks) : direct<false, 2, 2, 4, 2>(blocks); break;
             case 4: direct<false, 2, 4, 4, 2>(blocks); break;
-            case 5: hipLaunchKernelGGL((mx_tile_kernel<T, 128, 128, 2, 2, 4>), dim3(blocks), dim3(256), 0, stream(), p); break;
+            case 5: direct<false, 4, 4, 4, 2>(blocks); break;
+            case 6: hipLaunchKernelGGL((mx_tile_kernel<T, 128, 128, 2, 2, 4>), dim3(blocks), dim3(256), 0, stream(), p); break;
             default: hipLaunchKernelGGL((mx_tile_kernel<T, 256, 256, 4, 2, 4>), dim3(blocks), dim3(512), 0, stream(), p); break;
         }
         AGH_LAUNCH_CHECK(name);
@@ -120,7 +132,7 @@ int dense_entry(const char *name, int64_t m, int64_t k, int64_t n, const void *x
         if (int rc = check_operand(name, "w", w_codes, w_scales)) return rc;
         const int64_t steps = steps_of(k);
         const int form = choose_form(m, n, steps);
-        if (kForms[form].bq == 16 && csx == 1) {
+        if (csx == 1 && quantises_itself(form, m, n, steps)) {
             // few rows: quantised by every workgroup for itself, in one launch
             Launch<T> l = {name, {nullptr, nullptr, (const unsigned char *)w_codes, (const unsigned char *)w_scales, (T *)c + off_c, rsc, csc,
                                   bias ? (const T *)bias + off_bias : nullptr, bias_stride, (int)m, (int)n, (int)steps, act, false, 0, 0}, (const T *)x + off_x, rsx, (int)k};

@@ -51,7 +51,7 @@ __global__ __launch_bounds__(WGP * WGQ * 64) void mx_tile_kernel(Problem g) {
     constexpr int SCALES = (FP + FQ) * kFragBytes, STAGE = SCALES + (PP + PQ) * kPieceBytes;
     constexpr int NF = (FP + FQ) / NW, NP = (PP + PQ + NW - 1) / NW, NL = NF + NP;  // loads a wave issues for a step
     static_assert(WP % 64 == 0 && WQ % 64 == 0, "the rows of a wave are whole pieces");
-    static_assert((FP + FQ) % NW == 0 && (NS - 1) * NL < 64 && NS % 2 == 0, "");
+    static_assert((FP + FQ) % NW == 0 && (NS - 1) * NL < 64 && NS % 2 == 0, "every wave issues as many loads; the sets alternate with the stages");
     __shared__ __align__(16) unsigned char lds[NS * STAGE];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

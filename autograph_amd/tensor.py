@@ -104,10 +104,6 @@ def _dims(shape):
     return dims
 
 
-def _ptr_or_none(t):
-    return None if t is None else t._data_ptr()
-
-
 def _std_strides(shape):
     if len(shape) == 2:
         return (shape[1], 1)
@@ -408,53 +404,63 @@ class Tensor:
 
     # -- layer norm over the last axis (no counterpart in the reference) --
     def _norm_vector(self, v, name):
+        """The address of a weight or bias of layer norm, checked, and what keeps it alive until the call."""
         if v is None:
-            return None
+            return None, None
         if v.dtype != self.dtype or v.shape != self.shape[-1:]:
             raise AghError(-1, f"layer_norm: {name} must be a {self.dtype} vector of length {self.shape[-1]}")
-        return v.as_standard_layout()
+        v = v.as_standard_layout()
+        return v._data_ptr(), v
 
     def layer_norm(self, weight=None, bias=None, epsilon=1e-5, stats=False):
         """(x - mean) / sqrt(var + epsilon) * weight + bias over the last axis.  With `stats`: (y, mean, rstd), the f32 tensors that
         `layer_norm_backward` takes, one value a row."""
-        if self.ndim < 1:
+        shape, dtype = self.shape, self.dtype
+        if not shape:
             raise AghError(-1, "layer_norm: a tensor without axes")
         x = self.as_standard_layout()
-        w, b = self._norm_vector(weight, "weight"), self._norm_vector(bias, "bias")
-        lead = x.shape[:-1]
-        y = _uninit(x.shape, x.dtype)
-        mean, rstd = (_uninit(lead, F32), _uninit(lead, F32)) if stats else (None, None)
-        self._call("agh_layer_norm")(x._data_ptr(), _ptr_or_none(w), _ptr_or_none(b), epsilon, y._ptr(), _ptr_or_none(mean),
-                                     _ptr_or_none(rstd), math.prod(lead), x.shape[-1])
-        return (y, mean, rstd) if stats else y
+        w, _w = self._norm_vector(weight, "weight")
+        b, _b = self._norm_vector(bias, "bias")
+        y = _uninit(shape, dtype)
+        call = calls.agh_layer_norm_f32 if dtype == F32 else calls.agh_layer_norm_bf16
+        rows = shape[0] if len(shape) == 2 else math.prod(shape[:-1])
+        if not stats:
+            call(x._data_ptr(), w, b, epsilon, y.buffer.ptr, None, None, rows, shape[-1])
+            return y
+        mean, rstd = _uninit(shape[:-1], F32), _uninit(shape[:-1], F32)
+        call(x._data_ptr(), w, b, epsilon, y.buffer.ptr, mean.buffer.ptr, rstd.buffer.ptr, rows, shape[-1])
+        return y, mean, rstd
 
     def layer_norm_backward(self, output_grad, weight, mean, rstd):
         """Gradients (dx, dweight, dbias) of `self.layer_norm(weight, bias, stats=True)`, `self` being its input; with weight None
         (dx, None, None)."""
-        if self.ndim < 1:
+        shape, dtype = self.shape, self.dtype
+        if not shape:
             raise AghError(-1, "layer_norm_backward: a tensor without axes")
-        if output_grad.dtype != self.dtype or output_grad.shape != self.shape:
-            raise AghError(-1, f"layer_norm_backward: expected a {self.dtype} gradient of {self.shape}, found {output_grad.dtype} {output_grad.shape}")
-        lead = self.shape[:-1]
-        for name, v in (("mean", mean), ("rstd", rstd)):
-            if v.dtype != F32 or v.shape != lead:
-                raise AghError(-1, f"layer_norm_backward: {name} must be an f32 tensor of {lead}, found {v.dtype} {v.shape}")
+        if output_grad.dtype != dtype or output_grad.shape != shape:
+            raise AghError(-1, f"layer_norm_backward: expected a {dtype} gradient of {shape}, found {output_grad.dtype} {output_grad.shape}")
+        lead = shape[:-1]
+        if mean.dtype != F32 or rstd.dtype != F32 or mean.shape != lead or rstd.shape != lead:
+            raise AghError(-1, f"layer_norm_backward: mean and rstd must be f32 tensors of {lead}, found {mean.dtype} {mean.shape}, {rstd.dtype} {rstd.shape}")
         x, dy, mean, rstd = self.as_standard_layout(), output_grad.as_standard_layout(), mean.as_standard_layout(), rstd.as_standard_layout()
-        w = self._norm_vector(weight, "weight")
-        dx = _uninit(x.shape, x.dtype)
-        dw, db = (_uninit(x.shape[-1:], x.dtype), _uninit(x.shape[-1:], x.dtype)) if w is not None else (None, None)
-        self._call("agh_layer_norm_backward")(x._data_ptr(), dy._data_ptr(), _ptr_or_none(w), mean._data_ptr(), rstd._data_ptr(), dx._ptr(),
-                                              _ptr_or_none(dw), _ptr_or_none(db), math.prod(lead), x.shape[-1])
+        w, _w = self._norm_vector(weight, "weight")
+        dx = _uninit(shape, dtype)
+        dw, db = (None, None) if weight is None else (_uninit(shape[-1:], dtype), _uninit(shape[-1:], dtype))
+        call = calls.agh_layer_norm_backward_f32 if dtype == F32 else calls.agh_layer_norm_backward_bf16
+        call(x._data_ptr(), dy._data_ptr(), w, mean._data_ptr(), rstd._data_ptr(), dx.buffer.ptr, None if dw is None else dw.buffer.ptr,
+             None if db is None else db.buffer.ptr, shape[0] if len(shape) == 2 else math.prod(lead), shape[-1])
         return dx, dw, db
 
     # -- MXFP4 (no counterpart in the reference) --
     def quantize_mxfp4(self, axis=1):
         """The matrix in 4 bits, blocks of 32 along `axis`: the axis that a product will sum over (1 for a left operand, 0 for a right one)."""
-        if self.ndim != 2 or axis not in (0, 1):
-            raise AghError(-1, f"quantize_mxfp4: a matrix and axis 0 or 1 expected, found {self.shape} and {axis!r}")
-        out = MxTensor.uninit(self.shape, axis)
-        self._call("agh_quantize_mxfp4")(self._ptr(), self.offset, self.strides[1 - axis], self.strides[axis], self.shape[1 - axis], self.shape[axis],
-                                         out.codes.ptr, out.scales.ptr)
+        shape, strides = self.shape, self.strides
+        if len(shape) != 2 or axis not in (0, 1):
+            raise AghError(-1, f"quantize_mxfp4: a matrix and axis 0 or 1 expected, found {shape} and {axis!r}")
+        (rows, k), (rs, cs) = (shape, strides) if axis == 1 else (shape[::-1], strides[::-1])
+        out = MxTensor.uninit(shape, axis)
+        call = calls.agh_quantize_mxfp4_f32 if self.dtype == F32 else calls.agh_quantize_mxfp4_bf16
+        call(self.buffer.ptr, self.offset, rs, cs, rows, k, out.codes.ptr, out.scales.ptr)
         return out
 
     def cross_entropy_loss_backward(self, target, dy=1.0):
@@ -474,9 +480,9 @@ class MxTensor:
 
     @classmethod
     def uninit(cls, shape, axis):
-        rows, k = shape[1 - axis], shape[axis]
-        steps = -(-k // 128)
-        return cls(Buffer(-(-rows // 16) * steps * 1024), Buffer(-(-rows // 64) * steps * 256), shape, axis)
+        rows, k = shape if axis == 1 else shape[::-1]
+        steps = (k + 127) // 128
+        return cls(Buffer((rows + 15) // 16 * steps * 1024), Buffer((rows + 63) // 64 * steps * 256), shape, axis)
 
     def t(self):
         """The transposed matrix: no data moves, the blocks run along the other axis."""
@@ -488,7 +494,8 @@ class MxTensor:
             raise AghError(-1, f"dequantize: unknown type {dtype!r}")
         y = _uninit(self.shape, dtype)
         a = self.axis
-        y._call("agh_dequantize_mxfp4")(self.codes.ptr, self.scales.ptr, self.shape[1 - a], self.shape[a], y._ptr(), 0, y.strides[1 - a], y.strides[a])
+        call = calls.agh_dequantize_mxfp4_f32 if dtype == F32 else calls.agh_dequantize_mxfp4_bf16
+        call(self.codes.ptr, self.scales.ptr, self.shape[1 - a], self.shape[a], y.buffer.ptr, 0, y.strides[1 - a], y.strides[a])
         return y
 
     def dot(self, rhs, bias=None, relu=False, dtype=BF16):
@@ -503,8 +510,9 @@ class MxTensor:
         if bias is not None and (bias.dtype != dtype or bias.shape != (n,)):
             raise AghError(-1, f"bias must be a {dtype} vector of length {n}")
         out = _uninit((m, n), dtype)
-        bp, bo, bs_ = (bias._ptr(), bias.offset, bias.strides[0]) if bias is not None else (None, 0, 0)
-        out._call("agh_gemm_mxfp4")(m, k, n, self.codes.ptr, self.scales.ptr, rhs.codes.ptr, rhs.scales.ptr, out._ptr(), 0, n, 1, bp, bo, bs_, 1 if relu else 0)
+        bp, bo, bs_ = (None, 0, 0) if bias is None else (bias.buffer.ptr, bias.offset, bias.strides[0])
+        call = calls.agh_gemm_mxfp4_f32 if dtype == F32 else calls.agh_gemm_mxfp4_bf16
+        call(m, k, n, self.codes.ptr, self.scales.ptr, rhs.codes.ptr, rhs.scales.ptr, out.buffer.ptr, 0, n, 1, bp, bo, bs_, 1 if relu else 0)
         return out
 
     @staticmethod
