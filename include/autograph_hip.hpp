@@ -15,6 +15,7 @@
 #include <stdexcept>
 #include <string>
 #include <type_traits>
+#include <utility>
 #include <vector>
 
 #include "autograph_hip.h"
@@ -138,6 +139,9 @@ inline std::string shape_str(const Shape &d) {
 }
 
 template <typename T> class Tensor;
+class MxTensor;
+template <typename T> struct LayerNormed;     // result and statistics of Tensor::layer_norm_train
+template <typename T> struct LayerNormGrads;  // of Tensor::layer_norm_backward
 template <typename T> void gemm(float alpha, const Tensor<T> &a, const Tensor<T> &b, float beta, Tensor<T> &c,
                                 const Tensor<T> *bias = nullptr, bool relu = false);
 
@@ -343,6 +347,20 @@ public:
         check((kBf16 ? agh_sum_axis0_bf16 : agh_sum_axis0_f32)(x.data_ptr(), y.buffer_ptr(), dim_[0], dim_[1]));
         return y;
     }
+    // -- layer norm over the last axis (no counterpart in the reference); weight and bias [features], either null --
+    Tensor layer_norm(const Tensor *weight, const Tensor *bias, float epsilon = 1e-5f) const {
+        Tensor y = uninit(dim_);
+        layer_norm_into(weight, bias, epsilon, y, nullptr, nullptr);
+        return y;
+    }
+    // with the f32 statistics, one value a row, that layer_norm_backward takes
+    LayerNormed<T> layer_norm_train(const Tensor *weight, const Tensor *bias, float epsilon = 1e-5f) const;
+    // gradients with respect to *this (the input), weight and bias
+    LayerNormGrads<T> layer_norm_backward(const Tensor &output_grad, const Tensor &weight, const Tensor<float> &mean, const Tensor<float> &rstd) const;
+
+    // -- MXFP4 (no counterpart in the reference): blocks of 32 along `axis`, the one a product will sum over --
+    MxTensor quantize_mxfp4(int axis = 1) const;
+
     Tensor clone() const {
         const Tensor x = as_standard_layout();
         Tensor out = uninit(dim_);
@@ -351,6 +369,18 @@ public:
     }
 
 private:
+    template <typename U> friend class Tensor;
+    void check_features(const Tensor &v, const char *name) const {
+        if (v.ndim() != 1 || v.dim_[0] != dim_.back()) bail(std::string("layer_norm: ") + name + " must be a vector of length " + std::to_string(dim_.back()));
+    }
+    void layer_norm_into(const Tensor *weight, const Tensor *bias, float epsilon, Tensor &y, void *mean, void *rstd) const {
+        if (dim_.empty()) bail("layer_norm: a tensor without axes");
+        if (weight) check_features(*weight, "weight");
+        if (bias) check_features(*bias, "bias");
+        const Tensor x = as_standard_layout(), w = weight ? weight->as_standard_layout() : Tensor(), b = bias ? bias->as_standard_layout() : Tensor();
+        check((kBf16 ? agh_layer_norm_bf16 : agh_layer_norm_f32)(x.data_ptr(), weight ? w.data_ptr() : nullptr, bias ? b.data_ptr() : nullptr, epsilon,
+                                                                 y.buffer_ptr(), mean, rstd, shape_len(Shape(dim_.begin(), dim_.end() - 1)), dim_.back()));
+    }
     Tensor dot_impl(const Tensor &rhs, const Tensor *bias, bool relu) const {
         if (ndim() != 2 || rhs.ndim() != 2) bail("dot: both operands must be 2-D");
         Tensor out = uninit({dim_[0], rhs.dim_[1]});
@@ -382,6 +412,91 @@ void gemm(float alpha, const Tensor<T> &a, const Tensor<T> &b, float beta, Tenso
             b.strides()[1], beta, c.buffer_ptr(), c.offset(), c.strides()[0], c.strides()[1], bias ? bias->buffer_ptr() : nullptr,
             bias ? bias->offset() : 0, bias ? bias->strides()[0] : 0, relu ? AGH_ACT_RELU : AGH_ACT_NONE));
     }
+}
+
+template <typename T> struct LayerNormed {
+    Tensor<T> y;
+    Tensor<float> mean, rstd;
+};
+template <typename T> struct LayerNormGrads {
+    Tensor<T> input, weight, bias;
+};
+template <typename T> LayerNormed<T> Tensor<T>::layer_norm_train(const Tensor *weight, const Tensor *bias, float epsilon) const {
+    if (dim_.empty()) bail("layer_norm: a tensor without axes");
+    const Shape lead(dim_.begin(), dim_.end() - 1);
+    LayerNormed<T> out{uninit(dim_), Tensor<float>::uninit(lead), Tensor<float>::uninit(lead)};
+    layer_norm_into(weight, bias, epsilon, out.y, out.mean.buffer_ptr(), out.rstd.buffer_ptr());
+    return out;
+}
+template <typename T>
+LayerNormGrads<T> Tensor<T>::layer_norm_backward(const Tensor &output_grad, const Tensor &weight, const Tensor<float> &mean, const Tensor<float> &rstd) const {
+    if (dim_.empty()) bail("layer_norm_backward: a tensor without axes");
+    const Shape lead(dim_.begin(), dim_.end() - 1), features{dim_.back()};
+    if (output_grad.dim_ != dim_) bail("layer_norm_backward: expected a gradient of " + shape_str(dim_) + ", found " + shape_str(output_grad.dim_));
+    if (mean.shape() != lead || rstd.shape() != lead) bail("layer_norm_backward: mean and rstd must be " + shape_str(lead));
+    check_features(weight, "weight");
+    const Tensor x = as_standard_layout(), dy = output_grad.as_standard_layout(), w = weight.as_standard_layout();
+    const Tensor<float> m = mean.as_standard_layout(), r = rstd.as_standard_layout();
+    LayerNormGrads<T> out{uninit(dim_), uninit(features), uninit(features)};
+    check((kBf16 ? agh_layer_norm_backward_bf16 : agh_layer_norm_backward_f32)(x.data_ptr(), dy.data_ptr(), w.data_ptr(), m.data_ptr(), r.data_ptr(),
+                                                                               out.input.buffer_ptr(), out.weight.buffer_ptr(), out.bias.buffer_ptr(),
+                                                                               shape_len(lead), dim_.back()));
+    return out;
+}
+
+// A matrix in MXFP4: blocks of 32 values along `axis` share a scale, a power of two, and hold 4 bits each (agh_quantize_mxfp4_<T> says how they lie).
+class MxTensor {
+public:
+    MxTensor(int64_t rows, int64_t cols, int axis) : dim_{rows, cols}, axis_(axis) {
+        if (axis != 0 && axis != 1) bail("MxTensor: axis 0 or 1 expected");
+        size_t codes = 0, scales = 0;
+        check(agh_mxfp4_bytes(vectors(), values(), &codes, &scales));
+        codes_ = std::make_shared<Buffer<uint8_t>>(codes);
+        scales_ = std::make_shared<Buffer<uint8_t>>(scales);
+    }
+    const std::array<int64_t, 2> &shape() const { return dim_; }
+    int axis() const { return axis_; }
+    int64_t vectors() const { return dim_[1 - axis_]; }  // quantised along their `values`
+    int64_t values() const { return dim_[axis_]; }
+    void *codes() const { return codes_->ptr(); }
+    void *scales() const { return scales_->ptr(); }
+    // the transposed matrix: no data moves, the blocks run along the other axis
+    MxTensor t() const {
+        MxTensor out = *this;
+        std::swap(out.dim_[0], out.dim_[1]);
+        out.axis_ = 1 - axis_;
+        return out;
+    }
+    template <typename T> Tensor<T> dequantize() const {
+        Tensor<T> y = Tensor<T>::uninit({dim_[0], dim_[1]});
+        check((std::is_same<T, bf16>::value ? agh_dequantize_mxfp4_bf16 : agh_dequantize_mxfp4_f32)(codes(), scales(), vectors(), values(), y.buffer_ptr(), 0,
+                                                                                                    y.strides()[1 - axis_], y.strides()[axis_]));
+        return y;
+    }
+    // `Tensor::dot` of two quantised matrices, each along the axis that is summed over; bias and relu in the same launch, one rounding
+    template <typename T> Tensor<T> dot(const MxTensor &rhs, const Tensor<T> *bias = nullptr, bool relu = false) const {
+        if (axis_ != 1 || rhs.axis_ != 0) bail("dot: the left operand must be quantised along axis 1 and the right one along axis 0");
+        if (dim_[1] != rhs.dim_[0]) bail("a_cols != b_rows, " + std::to_string(dim_[1]) + " != " + std::to_string(rhs.dim_[0]));
+        const int64_t n = rhs.dim_[1];
+        if (bias && (bias->ndim() != 1 || bias->shape()[0] != n)) bail("bias must be a vector of length " + std::to_string(n));
+        Tensor<T> c = Tensor<T>::uninit({dim_[0], n});
+        check((std::is_same<T, bf16>::value ? agh_gemm_mxfp4_bf16 : agh_gemm_mxfp4_f32)(
+            dim_[0], dim_[1], n, codes(), scales(), rhs.codes(), rhs.scales(), c.buffer_ptr(), 0, n, 1, bias ? bias->buffer_ptr() : nullptr,
+            bias ? bias->offset() : 0, bias ? bias->strides()[0] : 0, relu ? AGH_ACT_RELU : AGH_ACT_NONE));
+        return c;
+    }
+
+private:
+    std::array<int64_t, 2> dim_;
+    int axis_;
+    std::shared_ptr<Buffer<uint8_t>> codes_, scales_;
+};
+template <typename T> MxTensor Tensor<T>::quantize_mxfp4(int axis) const {
+    if (ndim() != 2) bail("quantize_mxfp4: a matrix expected, found " + shape_str(dim_));
+    MxTensor out(dim_[0], dim_[1], axis);
+    check((kBf16 ? agh_quantize_mxfp4_bf16 : agh_quantize_mxfp4_f32)(buffer_ptr(), offset_, strides_[1 - axis], strides_[axis], dim_[1 - axis], dim_[axis],
+                                                                     out.codes(), out.scales()));
+    return out;
 }
 
 // ---- layers (src/learn/neural_network/layer.rs) ----
@@ -430,6 +545,29 @@ template <typename T> struct Dense {
         if (bias) out.add_assign(*bias);
         return relu ? out.relu() : out;
     }
+};
+// `Dense` with its weight [inputs, outputs] in MXFP4, quantised along the inputs: `MxDense<T>{dense.weight.quantize_mxfp4(0), dense.bias}`
+template <typename T> struct MxDense {
+    MxTensor weight;
+    std::shared_ptr<Tensor<T>> bias;
+    Tensor<T> forward(const Tensor<T> &input, bool relu = false) const {
+        if (input.ndim() != 2 || weight.axis() != 0) bail("MxDense: a 2-D input and a weight quantised along axis 0 expected");
+        const int64_t m = input.shape()[0], k = input.shape()[1], n = weight.shape()[1];
+        if (k != weight.shape()[0]) bail("a_cols != b_rows, " + std::to_string(k) + " != " + std::to_string(weight.shape()[0]));
+        if (bias && (bias->ndim() != 1 || bias->shape()[0] != n)) bail("bias must be a vector of length " + std::to_string(n));
+        Tensor<T> y = Tensor<T>::uninit({m, n});
+        check((std::is_same<T, bf16>::value ? agh_dense_mxfp4_bf16 : agh_dense_mxfp4_f32)(
+            m, k, n, input.buffer_ptr(), input.offset(), input.strides()[0], input.strides()[1], weight.codes(), weight.scales(), y.buffer_ptr(), 0, n, 1,
+            bias ? bias->buffer_ptr() : nullptr, bias ? bias->offset() : 0, bias ? bias->strides()[0] : 0, relu ? AGH_ACT_RELU : AGH_ACT_NONE));
+        return y;
+    }
+};
+// Layer norm over the last axis: weight and bias [features], either may be empty
+template <typename T> struct LayerNorm {
+    std::shared_ptr<Tensor<T>> weight, bias;
+    float epsilon = 1e-5f;
+    Tensor<T> forward(const Tensor<T> &input) const { return input.layer_norm(weight.get(), bias.get(), epsilon); }
+    LayerNormed<T> forward_train(const Tensor<T> &input) const { return input.layer_norm_train(weight.get(), bias.get(), epsilon); }
 };
 // `MaxPool2` (layer.rs:1149-1216); the stride defaults to the filter (layer.rs:535-539)
 template <typename T> struct MaxPool2 {
