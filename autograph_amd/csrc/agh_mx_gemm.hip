@@ -12,18 +12,18 @@ using namespace agh::mx;
 namespace {
 
 // The kernels' tiles (p: columns of c, q: rows) and what a product takes in them, fitted to measured times in us: `start`, and for each tile that a CU takes in turn
-// `tile` + `step` for every 128 of k, but at least `least` (fetching the kernel's code, storing the result).  Measured against the estimate: 1x4096x4096 3.7 /
-// 3.8 (16x16), 32x4096x4096 4.1 / 4.1 (16x32), 64x4096x4096 5.5 / 5.4 (32x32), 512x2048x2048 6.5 / 6.9 (32x64), 1024x4096x1024 7.9 / 7.8 (64x64),
-// 1999x2047x1001 9.3 / 9.3 (128x128), 16384x4096x4096 125 / 116 (256x256).  Over 220 products of sizes drawn at random the form chosen takes 1.02 of the best one's time in
-// the mean.  (128x128 tiles with k split between two halves of a workgroup took 11.5 instead of 12.4 us at 2048x4096x1000 and lost where k is short; not taken.)
+// `tile` (half as much again for f32 results of the large tiles, which they are bound by) + `step` for every 128 of k, but at least `least` (fetching the kernel's code,
+// storing the result).  Over 520 products, sizes drawn at random, both types, no operand in a cache from the call before, the form chosen takes 1.02 of the best one's
+// time in the mean, and more than 1.12 of it in 4 of 100.  (128x128 tiles with k split between two halves of a workgroup took 11.5 instead of 12.4 us at 2048x4096x1000
+// and lost where k is short; not taken.)
 struct Form {
     int bp, bq;
     double start, tile, step, least;
 };
-constexpr Form kForms[] = {{16, 16, 2.5, 0.2, 0.034, 0.4},  {32, 16, 2.5, 0.2, 0.064, 0.5}, {16, 32, 2.7, 0.2, 0.039, 0.62},   {32, 32, 2.7, 0.16, 0.08, 0.6},
-                           {32, 64, 3.0, 0.7, 0.075, 1.25}, {64, 64, 3.2, 2.0, 0.08, 2.7},  {128, 128, 4.0, 1.9, 0.2125, 0.0}, {256, 256, 4.0, 6.2, 0.68, 0.0}};
+constexpr Form kForms[] = {{16, 16, 2.5, 0.2, 0.034, 0.4},   {32, 16, 2.5, 0.2, 0.064, 0.5},   {16, 32, 3.1, 0.13, 0.042, 0.73}, {32, 32, 2.5, 0.2, 0.071, 0.48},
+                           {32, 64, 3.6, 0.65, 0.077, 1.25}, {64, 64, 3.2, 2.66, 0.174, 2.7}, {128, 128, 4.0, 1.6, 0.19, 0.0},  {256, 256, 2.8, 5.9, 0.54, 0.0}};
 
-int choose_form(int64_t m, int64_t n, int64_t steps) {
+int choose_form(int64_t m, int64_t n, int64_t steps, size_t element) {
     int best = 0;
     double least = 1e30;
     for (int f = 0; f < (int)(sizeof(kForms) / sizeof(kForms[0])); ++f) {
@@ -31,8 +31,9 @@ int choose_form(int64_t m, int64_t n, int64_t steps) {
         if (o.bq == 16 && m > 16) continue;
         const double tiles = (double)((n + o.bp - 1) / o.bp) * (double)((m + o.bq - 1) / o.bq), cus = compute_units();
         // the tiled kernels' workgroups fill a CU, one or two at a time; many small ones share it evenly
-        const double turns = o.bp >= 128 ? (double)(int64_t)((tiles + cus - 1) / cus) : tiles > cus ? tiles / cus : 1.0;
-        const double each = o.tile + o.step * (double)steps, us = o.start + turns * (each > o.least ? each : o.least);
+        const bool large = o.bp >= 128;
+        const double turns = large ? (double)(int64_t)((tiles + cus - 1) / cus) : tiles > cus ? tiles / cus : 1.0;
+        const double each = o.tile * (large && element == 4 ? 1.5 : 1.0) + o.step * (double)steps, us = o.start + turns * (each > o.least ? each : o.least);
         if (us < least) least = us, best = f;
     }
     return best;
@@ -118,7 +119,7 @@ int gemm_entry(const char *name, int64_t m, int64_t k, int64_t n, const void *a_
     const int64_t steps = steps_of(k);
     Launch<T> l = {name, {(const unsigned char *)a_codes, (const unsigned char *)a_scales, (const unsigned char *)b_codes, (const unsigned char *)b_scales,
                           (T *)c + off_c, rsc, csc, bias ? (const T *)bias + off_bias : nullptr, bias_stride, (int)m, (int)n, (int)steps, act, rows_aligned<T>((T *)c + off_c, rsc), 0, 0}, nullptr, 0, 0};
-    return l.run(choose_form(m, n, steps));
+    return l.run(choose_form(m, n, steps, sizeof(T)));
 }
 
 template <typename T>
@@ -131,7 +132,7 @@ int dense_entry(const char *name, int64_t m, int64_t k, int64_t n, const void *x
         if (!x) return fail(AGH_ENULL, "%s: null input", name);
         if (int rc = check_operand(name, "w", w_codes, w_scales)) return rc;
         const int64_t steps = steps_of(k);
-        const int form = choose_form(m, n, steps);
+        const int form = choose_form(m, n, steps, sizeof(T));
         if (csx == 1 && quantises_itself(form, m, n, steps)) {
             // few rows: quantised by every workgroup for itself, in one launch
             Launch<T> l = {name, {nullptr, nullptr, (const unsigned char *)w_codes, (const unsigned char *)w_scales, (T *)c + off_c, rsc, csc,
