@@ -170,9 +170,9 @@ __global__ __launch_bounds__(wg_threads(TPR)) void layer_norm_kernel(const T *x,
 
 // Backward: dx, and this workgroup's shares of dw and db.  shares [gridDim.x][2][pitch]: f32, or with one workgroup nothing, then dw and db are written here.
 template <typename T, int THREADS, int TPR, int VPT>
-__global__ __launch_bounds__(THREADS) void layer_norm_backward_kernel(const T *x, const T *dy, const T *__restrict__ w, const float *__restrict__ mean_in,
-                                                                      const float *__restrict__ rstd_in, T *dx, float *__restrict__ shares, T *__restrict__ dw,
-                                                                      T *__restrict__ db, int64_t rows, int cols, int pitch) {
+__global__ __launch_bounds__(THREADS, THREADS == 512 && VPT == 2 ? 4 : 1) void layer_norm_backward_kernel(
+    const T *x, const T *dy, const T *__restrict__ w, const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
+    T *dx, float *__restrict__ shares, T *__restrict__ dw, T *__restrict__ db, int64_t rows, int cols, int pitch) {
     using G = Group<T>;
     constexpr int VE = G::VE, ROWS = THREADS / TPR;
     static_assert(TPR <= 64 || ROWS == 1, "the waves of a row meet at the workgroup's barrier");
@@ -443,8 +443,10 @@ struct Backward {
         constexpr int per_wg = THREADS / TPR;
         // A workgroup's shares of dw and db, written and read again, cost what two to four rows do: no more workgroups than keep memory busy (bf16
         // 16384x4096, 512 threads: 256 workgroups 98.5 us, 512 76.6, 1024 87.7; 4096x16384: 256 89.8, 512 97.7), and two turns each at least.
-        const int64_t turns = (rows + per_wg - 1) / per_wg, most = (int64_t)compute_units() * (TPR <= 64 ? VPT <= 2 ? 3 : 2 : VPT <= 2 ? 2 : 1);
-        int64_t wgs = THREADS == 1024 ? 1 : (turns + 1) / 2;
+        // Where a quarter of the threads has no columns, a third fills the gap (512 threads by 1, f32 21845x1536 86.2 -> 78.5, bf16 13107x2560 55.6 -> 53.1; all at work, 8192x4096 bf16 46.2 -> 47.4).
+        const bool gaps = cols <= TPR * VPT * Group<T>::VE / 4 * 3;
+        const int64_t turns = (rows + per_wg - 1) / per_wg, most = (int64_t)compute_units() * (TPR <= 64 ? VPT <= 2 ? 3 : 2 : TPR == 512 && VPT <= 2 ? VPT == 1 && gaps ? 3 : 2 : 1);
+        int64_t wgs = THREADS == 1024 && TPR <= 64 ? 1 : (turns + 1) / 2;
         if (wgs > most) wgs = most;
         float *shares = nullptr;
         if (wgs > 1 && (dw || db))
@@ -495,12 +497,17 @@ int backward_entry(const char *name, const void *x, const void *dy, const void *
     if (groups <= 192) return f.template run<256, 64, 3>();
     if (groups <= 256) return f.template run<256, 64, 4>();
     if (groups <= 512) return f.template run<512, 512, 1>();
-    if (groups <= 1024) return f.template run<512, 512, 2>();
+    // (bf16 4096x8192: 512 threads with 2 in 135 registers, one workgroup a unit, 62.8 us; in 128, two, 53.0; 1024 threads 49.9.  5461x6144: 62.2, 53.7, 52.9; 7281x4608: 71.7, 55.6, 60.5.
+    // f32 8192x4096: 512 threads 69.3, 1024 76.7)
+    if (groups <= (VE == 8 ? 768 : 1024)) return f.template run<512, 512, 2>();
+    if (groups <= 1024) return f.template run<1024, 1024, 1>();
     if (groups <= 1536) return f.template run<512, 512, 3>();
     if (groups <= 2048) return f.template run<512, 512, 4>();
-    // (8 groups of bf16 a thread, with 128 sums, leave the compiler no registers)
-    if constexpr (VE == 4)
+    // (bf16 has twice the sums for each group, which leaves the compiler no registers: 1638x20480 190 us against 144 when the rows are read again)
+    if constexpr (VE == 4) {
+        if (groups <= 3 * 1024) return f.template run<1024, 1024, 3>();  // f32 3276x10240 85.7 us, 512 threads with 8 96
         if (groups <= 4096) return f.template run<512, 512, 8>();
+    }
     return f.run_long();
 }
 

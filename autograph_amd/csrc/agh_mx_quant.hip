@@ -112,11 +112,12 @@ __device__ __forceinline__ void decode(uint32_t c, float by, float &lo, float &h
     hi = v[1] * by;
 }
 
-// y's rows contiguous: a wave takes a fragment and writes whole rows of it, 128 values each, 16 bytes a lane.  Whole aligned groups leave with the streaming hint
-// (16384x4096 bf16 36.4 -> 26.1 us, f32 68 -> 48.7, 4096x4096 bf16 10.4 -> 8.4; unaligned ones lose by it, 16384x1001 bf16 12.8 -> 15.0).
+// y's rows contiguous: a wave takes a fragment and writes whole rows of it, 128 values each, 16 bytes a lane.  Rows on whole lines of memory leave with the streaming
+// hint (16384x4096 bf16 36.4 -> 26.1 us, f32 68 -> 48.7, 4096x4096 bf16 10.4 -> 8.4); of others two waves share lines, and they lose by it (bf16 16384x1032 9.0 -> 12.8,
+// f32 4096x2056 8.2 -> 10.2) or gain little (f32 16384x4104 77 -> 70).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void dequantize_rows_kernel(const unsigned char *__restrict__ codes, const unsigned char *__restrict__ scales, int rows,
-                                                                   int k, int steps, int64_t frags, T *__restrict__ y, int64_t rs, bool aligned) {
+                                                                   int k, int steps, int64_t frags, T *__restrict__ y, int64_t rs, bool streamed) {
     constexpr int VE = 16 / (int)sizeof(T), LANES = kStep / VE, ROWS = 64 / LANES;  // values a lane, lanes a row, rows a store instruction
     typedef typename std::conditional<VE == 8, uint32_t, uint16_t>::type Codes;     // of VE values
     const int64_t frag = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
@@ -144,7 +145,7 @@ __global__ __launch_bounds__(kThreads) void dequantize_rows_kernel(const unsigne
         for (int j = 0; j < VE; ++j) u.e[j] = Elem<T>::from_f32(f[j]);
         if (row >= rows || k0 >= k) continue;
         T *to = y + row * rs + k0;
-        if (aligned && k0 + VE <= k) __builtin_nontemporal_store(u.q, (u32x4_t *)to);
+        if (streamed && k0 + VE <= k) __builtin_nontemporal_store(u.q, (u32x4_t *)to);
         else if (k0 + VE <= k) *(typename Unaligned<T>::vec *)to = u.q;
         else
 #pragma unroll
@@ -214,7 +215,7 @@ int dequantize_entry(const char *name, const void *codes, const void *scales, in
     if (int rc = waves_grid(name, items, blocks)) return rc;
     if (cs == 1)
         hipLaunchKernelGGL(dequantize_rows_kernel<T>, dim3(blocks), dim3(kThreads), 0, stream(), c, s, (int)rows, (int)k, steps, items, to, rs,
-                           ((uintptr_t)to & 15) == 0 && rs * (int64_t)sizeof(T) % 16 == 0);
+                           ((uintptr_t)to | (uint64_t)rs * sizeof(T)) % 128 == 0);
     else
         hipLaunchKernelGGL(dequantize_strided_kernel<T>, dim3(blocks), dim3(kThreads), 0, stream(), c, s, (int)rows, (int)k, steps, items, to, rs, cs);
     AGH_LAUNCH_CHECK(name);

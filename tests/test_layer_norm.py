@@ -150,6 +150,14 @@ def test_layer_norm(ag, dtype, rows, cols):
 
 @gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(1700, 1300), (1600, 2600), (1100, 4090), (600, 7001), (530, 10250)])
+def test_layer_norm_many_wide_rows(ag, dtype, rows, cols):
+    """Several rows for each workgroup, at widths that a whole workgroup shares."""
+    test_layer_norm(ag, dtype, rows, cols)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_without_weight_or_bias(ag, dtype):
     rng = np.random.default_rng(5)
     x, w, b, dy = make(rng, 12, 100, dtype)
