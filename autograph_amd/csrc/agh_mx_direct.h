@@ -79,6 +79,12 @@ __global__ __launch_bounds__(WK * 64) void mx_direct_kernel(Problem g, const T *
                 xq[c] >>= shift_q;
             }
             xp[c] >>= shift_p;
+            mfma_written(xp[c]);
+            mfma_written(xq[c]);
+            if constexpr (RAW)
+#pragma unroll
+                for (int j = 0; j < TQ; ++j) mfma_written(vq[c][j]);
+            mfma_ready();
             agh::gemm::static_for<TP>([&](auto ic) {
                 agh::gemm::static_for<TQ>([&](auto jc) {
                     constexpr int i = decltype(ic)::value, j = decltype(jc)::value;
@@ -86,11 +92,11 @@ __global__ __launch_bounds__(WK * 64) void mx_direct_kernel(Problem g, const T *
                 });
             });
         }
+        mfma_done(acc);  // (here and not behind the loops: between them the compiler may move accumulators)
     };
     int s = first;
     for (; s + U <= last; s += U) steps(s, std::integral_constant<int, U>{});
     for (; s < last; ++s) steps(s, std::integral_constant<int, 1>{});
-    mfma_done();
 #pragma unroll
     for (int i = 0; i < TP; ++i)
 #pragma unroll

@@ -32,8 +32,21 @@ __device__ __forceinline__ void mfma(f32x4_t &c, u32x4_t p, u32x4_t q, uint32_t 
                  : "+a"(c)
                  : "v"(p), "v"(q), "v"(sp), "v"(sq), "n"(SP & 1), "n"(SQ & 1), "n"(SP >> 1), "n"(SQ >> 1));
 }
-// behind the last of them, before the accumulators are read: the compiler does not know that they are results of matrix instructions
-__device__ __forceinline__ void mfma_done() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
+// The compiler does not see matrix instructions in these, so what it keeps to around its own is kept to here.
+// Operands that vector instructions wrote: two wait states before the first matrix instruction that reads them.  Each operand passes through the wait, so what writes it
+// stays in front.
+__device__ __forceinline__ void mfma_ready() { asm volatile("s_nop 1" ::: "memory"); }
+template <typename V>
+__device__ __forceinline__ void mfma_written(V &operand) { asm volatile("" : "+v"(operand)); }
+// Behind the last of them, before the accumulators are read: their passes, which are 8 at most.  The accumulators pass through it too.
+template <int N, int M>
+__device__ __forceinline__ void mfma_done(f32x4_t (&acc)[N][M]) {
+    asm volatile("s_nop 15" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < M; ++j) asm volatile("" : "+a"(acc[i][j]));
+}
 
 // 16 (4) bytes a lane from a wave-uniform address plus a lane's offset to LDS, lane after lane; awaited by s_waitcnt vmcnt
 __device__ __forceinline__ void load_fragment(const unsigned char *base, uint32_t lane16, uint32_t lds) {
@@ -165,7 +178,7 @@ __global__ __launch_bounds__(WGP * WGQ * 64) void mx_tile_kernel(Problem g) {
         });
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     }
-    mfma_done();
+    mfma_done(acc);
     __syncthreads();  // the stages are free: no load is in flight, no wave reads
 
     // Element r of lane l of acc[i][j] is D[p0 + wp WP + 16 i + 4 (l / 16) + r][q0 + wq WQ + 16 j + l % 16]: four neighbours in a row of c, the 16 lanes of a group in as
