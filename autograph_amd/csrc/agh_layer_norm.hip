@@ -261,31 +261,33 @@ __global__ __launch_bounds__(THREADS, THREADS == 512 && VPT == 2 ? 4 : 1) void l
     }
 }
 
-// dw (blockIdx.y 0) and db out of n workgroups' shares: a workgroup adds 16 columns, 4 threads of 4 columns by 64 parts of the shares
+// dw (blockIdx.y 0) and db out of n workgroups' shares: a workgroup adds 16 columns at a time, 4 threads of 4 columns by 64 parts of the shares
 template <typename T>
 __global__ __launch_bounds__(kThreads) void add_shares_kernel(const float *__restrict__ shares, int n, int pitch, T *__restrict__ dw, T *__restrict__ db, int cols) {
     __shared__ f32x4_t part[kThreads / 64][4];
     const int c = threadIdx.x & 3, p = threadIdx.x >> 2;
-    const int64_t col = (int64_t)blockIdx.x * 16 + c * 4;
     T *out = blockIdx.y ? db : dw;
     if (!out) return;
-    f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (col < cols) {
-        const float *from = shares + blockIdx.y * (int64_t)pitch + col;
+    for (int64_t col = (int64_t)blockIdx.x * 16 + c * 4; col - c * 4 < cols; col += (int64_t)gridDim.x * 16) {
+        f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (col < cols) {
+            const float *from = shares + blockIdx.y * (int64_t)pitch + col;
 #pragma unroll 8
-        for (int i = p; i < n; i += 64) s += *(const f32x4_t *)(from + (int64_t)i * 2 * pitch);
+            for (int i = p; i < n; i += 64) s += *(const f32x4_t *)(from + (int64_t)i * 2 * pitch);
+        }
+#pragma unroll
+        for (int d = 4; d < 64; d *= 2)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] += __shfl_xor(s[i], d);
+        __syncthreads();  // the turn before has been read
+        if ((threadIdx.x & 63) < 4) part[threadIdx.x >> 6][c] = s;
+        __syncthreads();
+        if (threadIdx.x >= 4 || col >= cols) continue;
+        s = part[0][c];
+#pragma unroll
+        for (int i = 1; i < kThreads / 64; ++i) s += part[i][c];
+        for (int i = 0; i < 4 && col + i < cols; ++i) out[col + i] = Elem<T>::from_f32(s[i]);
     }
-#pragma unroll
-    for (int d = 4; d < 64; d *= 2)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[i] += __shfl_xor(s[i], d);
-    if ((threadIdx.x & 63) < 4) part[threadIdx.x >> 6][c] = s;
-    __syncthreads();
-    if (threadIdx.x >= 4 || col >= cols) return;
-    s = part[0][c];
-#pragma unroll
-    for (int i = 1; i < kThreads / 64; ++i) s += part[i][c];
-    for (int i = 0; i < 4 && col + i < cols; ++i) out[col + i] = Elem<T>::from_f32(s[i]);
 }
 
 // ---- rows longer than a workgroup's registers hold: read again for every sum, from the caches where they fit ----
@@ -301,56 +303,59 @@ __device__ __forceinline__ float workgroup_sum(float v, float *part) {
 }
 
 constexpr int kLongThreads = 1024;
+constexpr int64_t kMostWorkgroups = 1 << 20;  // of a launch (its work items are counted in 32 bits): what lies behind takes further turns
 
 template <typename T>
 __global__ __launch_bounds__(kLongThreads) void layer_norm_long_kernel(const T *x, const T *__restrict__ w, const T *__restrict__ b, float eps, T *y,
-                                                                       float *__restrict__ mean_out, float *__restrict__ rstd_out, int cols) {
+                                                                       float *__restrict__ mean_out, float *__restrict__ rstd_out, int64_t rows, int cols) {
     __shared__ float part[kLongThreads / 64];
-    const int64_t row = blockIdx.x;
-    x += row * cols;
-    y += row * cols;
     const float per = 1.0f / (float)cols;
-    float s = 0.0f;
-    for (int64_t i = threadIdx.x; i < cols; i += kLongThreads) s += Elem<T>::raw(x[i]);
-    const float mean = workgroup_sum(s, part) * per;
-    s = 0.0f;
-    for (int64_t i = threadIdx.x; i < cols; i += kLongThreads) {
-        const float d = Elem<T>::raw(x[i]) - mean;
-        s += d * d;
-    }
-    const float rstd = 1.0f / sqrtf(workgroup_sum(s, part) * per + eps);
-    for (int64_t i = threadIdx.x; i < cols; i += kLongThreads) {
-        float v = (Elem<T>::raw(x[i]) - mean) * rstd;
-        if (w) v *= Elem<T>::raw(w[i]);
-        if (b) v += Elem<T>::raw(b[i]);
-        y[i] = Elem<T>::from_f32(v);
-    }
-    if (threadIdx.x == 0) {
-        if (mean_out) mean_out[row] = mean;
-        if (rstd_out) rstd_out[row] = rstd;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const T *xr = x + row * cols;
+        T *yr = y + row * cols;
+        float s = 0.0f;
+        for (int64_t i = threadIdx.x; i < cols; i += kLongThreads) s += Elem<T>::raw(xr[i]);
+        const float mean = workgroup_sum(s, part) * per;
+        s = 0.0f;
+        for (int64_t i = threadIdx.x; i < cols; i += kLongThreads) {
+            const float d = Elem<T>::raw(xr[i]) - mean;
+            s += d * d;
+        }
+        const float rstd = 1.0f / sqrtf(workgroup_sum(s, part) * per + eps);
+        for (int64_t i = threadIdx.x; i < cols; i += kLongThreads) {
+            float v = (Elem<T>::raw(xr[i]) - mean) * rstd;
+            if (w) v *= Elem<T>::raw(w[i]);
+            if (b) v += Elem<T>::raw(b[i]);
+            yr[i] = Elem<T>::from_f32(v);
+        }
+        if (threadIdx.x == 0) {
+            if (mean_out) mean_out[row] = mean;
+            if (rstd_out) rstd_out[row] = rstd;
+        }
     }
 }
 
 template <typename T>
 __global__ __launch_bounds__(kLongThreads) void layer_norm_backward_long_kernel(const T *x, const T *dy, const T *__restrict__ w, const float *__restrict__ mean_in,
-                                                                                const float *__restrict__ rstd_in, T *dx, int cols) {
+                                                                                const float *__restrict__ rstd_in, T *dx, int64_t rows, int cols) {
     __shared__ float part[kLongThreads / 64];
-    const int64_t row = blockIdx.x;
-    const float mean = mean_in[row], rstd = rstd_in[row], per = 1.0f / (float)cols;
-    x += row * cols;
-    dy += row * cols;
-    dx += row * cols;
-    float sg = 0.0f, sgh = 0.0f;
-    for (int64_t i = threadIdx.x; i < cols; i += kLongThreads) {
-        const float g = Elem<T>::raw(dy[i]) * (w ? Elem<T>::raw(w[i]) : 1.0f);
-        sg += g;
-        sgh += g * ((Elem<T>::raw(x[i]) - mean) * rstd);
-    }
-    sg = workgroup_sum(sg, part) * per;
-    sgh = workgroup_sum(sgh, part) * per;
-    for (int64_t i = threadIdx.x; i < cols; i += kLongThreads) {
-        const float g = Elem<T>::raw(dy[i]) * (w ? Elem<T>::raw(w[i]) : 1.0f);
-        dx[i] = Elem<T>::from_f32(rstd * (g - sg - (Elem<T>::raw(x[i]) - mean) * rstd * sgh));
+    const float per = 1.0f / (float)cols;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const float mean = mean_in[row], rstd = rstd_in[row];
+        const T *xr = x + row * cols, *dyr = dy + row * cols;
+        T *dxr = dx + row * cols;
+        float sg = 0.0f, sgh = 0.0f;
+        for (int64_t i = threadIdx.x; i < cols; i += kLongThreads) {
+            const float g = Elem<T>::raw(dyr[i]) * (w ? Elem<T>::raw(w[i]) : 1.0f);
+            sg += g;
+            sgh += g * ((Elem<T>::raw(xr[i]) - mean) * rstd);
+        }
+        sg = workgroup_sum(sg, part) * per;
+        sgh = workgroup_sum(sgh, part) * per;
+        for (int64_t i = threadIdx.x; i < cols; i += kLongThreads) {
+            const float g = Elem<T>::raw(dyr[i]) * (w ? Elem<T>::raw(w[i]) : 1.0f);
+            dxr[i] = Elem<T>::from_f32(rstd * (g - sg - (Elem<T>::raw(xr[i]) - mean) * rstd * sgh));
+        }
     }
 }
 
@@ -419,7 +424,8 @@ int forward_entry(const char *name, const void *x, const void *w, const void *b,
     else if (groups <= 2048) f.template run<512, 4>();
     else if (groups <= 4096) f.template run<1024, 4>();
     else
-        hipLaunchKernelGGL(layer_norm_long_kernel<T>, dim3((unsigned)rows), dim3(kLongThreads), 0, stream(), f.x, f.w, f.b, eps, f.y, f.mean, f.rstd, f.cols);
+        hipLaunchKernelGGL(layer_norm_long_kernel<T>, dim3((unsigned)(rows < kMostWorkgroups ? rows : kMostWorkgroups)), dim3(kLongThreads), 0, stream(), f.x, f.w, f.b, eps, f.y,
+                           f.mean, f.rstd, rows, f.cols);
     AGH_LAUNCH_CHECK(name);
     return AGH_OK;
 }
@@ -434,7 +440,8 @@ struct Backward {
     int cols, pitch;
 
     int add(const float *shares, int64_t n) const {
-        hipLaunchKernelGGL(add_shares_kernel<T>, dim3((unsigned)((cols + 15) / 16), 2), dim3(kThreads), 0, stream(), shares, (int)n, pitch, dw, db, cols);
+        const int64_t wgs = ((int64_t)cols + 15) / 16;
+        hipLaunchKernelGGL(add_shares_kernel<T>, dim3((unsigned)(wgs < kMostWorkgroups ? wgs : kMostWorkgroups), 2), dim3(kThreads), 0, stream(), shares, (int)n, pitch, dw, db, cols);
         AGH_LAUNCH_CHECK(name);
         return AGH_OK;
     }
@@ -467,7 +474,8 @@ struct Backward {
             if (int rc = add(shares, n)) return rc;
         }
         if (dx) {
-            hipLaunchKernelGGL(layer_norm_backward_long_kernel<T>, dim3((unsigned)rows), dim3(kLongThreads), 0, stream(), x, dy, w, mean, rstd, dx, cols);
+            hipLaunchKernelGGL(layer_norm_backward_long_kernel<T>, dim3((unsigned)(rows < kMostWorkgroups ? rows : kMostWorkgroups)), dim3(kLongThreads), 0, stream(), x, dy, w,
+                               mean, rstd, dx, rows, cols);
             AGH_LAUNCH_CHECK(name);
         }
         return AGH_OK;

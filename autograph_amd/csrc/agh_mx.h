@@ -26,8 +26,10 @@ inline int64_t steps_of(int64_t k) { return (k + kStep - 1) / kStep; }
 inline size_t codes_bytes(int64_t rows, int64_t k) { return (size_t)((rows + 15) / 16) * (size_t)steps_of(k) * kFragBytes; }
 inline size_t scales_bytes(int64_t rows, int64_t k) { return (size_t)((rows + 63) / 64) * (size_t)steps_of(k) * kPieceBytes; }
 
-// rows and k of a quantised matrix: int indexes of fragments, rows and k
-inline bool sizes_fit(int64_t rows, int64_t k) { return rows < ((int64_t)1 << 31) - 512 && k < ((int64_t)1 << 31) - 512; }
+// rows and k of a quantised matrix: int indexes of fragments, rows and k, and a workgroup of 256 for each 64 rows x 128 k (a launch counts its work items in 32 bits)
+inline bool sizes_fit(int64_t rows, int64_t k) {
+    return rows < ((int64_t)1 << 31) - 512 && k < ((int64_t)1 << 31) - 512 && (rows + 63) / 64 * steps_of(k) < (1 << 24);
+}
 
 // quantises x (rows x k, element strides) into codes and scales on the current stream; arguments have been checked
 template <typename T>

@@ -17,19 +17,23 @@ namespace {
 // time in the mean, and more than 1.12 of it in 4 of 100.  (128x128 tiles with k split between two halves of a workgroup took 11.5 instead of 12.4 us at 2048x4096x1000
 // and lost where k is short; not taken.)
 struct Form {
-    int bp, bq;
+    int bp, bq, threads;
     double start, tile, step, least;
 };
-constexpr Form kForms[] = {{16, 16, 2.5, 0.2, 0.034, 0.4},   {32, 16, 2.5, 0.2, 0.064, 0.5},   {16, 32, 3.1, 0.13, 0.042, 0.73}, {32, 32, 2.5, 0.2, 0.071, 0.48},
-                           {32, 64, 3.6, 0.65, 0.077, 1.25}, {64, 64, 3.2, 2.66, 0.174, 2.7}, {128, 128, 4.0, 1.6, 0.19, 0.0},  {256, 256, 2.8, 5.9, 0.54, 0.0}};
+constexpr Form kForms[] = {{16, 16, 512, 2.5, 0.2, 0.034, 0.4},   {32, 16, 512, 2.5, 0.2, 0.064, 0.5},   {16, 32, 512, 3.1, 0.13, 0.042, 0.73},
+                           {32, 32, 256, 2.5, 0.2, 0.071, 0.48},  {32, 64, 256, 3.6, 0.65, 0.077, 1.25}, {64, 64, 256, 3.2, 2.66, 0.174, 2.7},
+                           {128, 128, 256, 4.0, 1.6, 0.19, 0.0},  {256, 256, 512, 2.8, 5.9, 0.54, 0.0}};
+constexpr int kFormCount = sizeof(kForms) / sizeof(kForms[0]);
+int64_t tiles_of(const Form &o, int64_t m, int64_t n) { return ((n + o.bp - 1) / o.bp) * ((m + o.bq - 1) / o.bq); }
+bool launches(const Form &o, int64_t m, int64_t n) { return tiles_of(o, m, n) <= 0xFFFFFFFFll / o.threads; }  // a launch counts its work items in 32 bits
 
 int choose_form(int64_t m, int64_t n, int64_t steps, size_t element) {
-    int best = 0;
+    int best = kFormCount - 1;
     double least = 1e30;
-    for (int f = 0; f < (int)(sizeof(kForms) / sizeof(kForms[0])); ++f) {
+    for (int f = 0; f < kFormCount; ++f) {
         const Form &o = kForms[f];
-        if (o.bq == 16 && m > 16) continue;
-        const double tiles = (double)((n + o.bp - 1) / o.bp) * (double)((m + o.bq - 1) / o.bq), cus = compute_units();
+        if ((o.bq == 16 && m > 16) || !launches(o, m, n)) continue;
+        const double tiles = (double)tiles_of(o, m, n), cus = compute_units();
         // the tiled kernels' workgroups fill a CU, one or two at a time; many small ones share it evenly
         const bool large = o.bp >= 128;
         const double turns = large ? (double)(int64_t)((tiles + cus - 1) / cus) : tiles > cus ? tiles / cus : 1.0;
@@ -45,7 +49,7 @@ int choose_form(int64_t m, int64_t n, int64_t steps, size_t element) {
 bool quantises_itself(int form, int64_t m, int64_t n, int64_t steps) {
     const Form &o = kForms[form];
     if (o.bq == 16) return true;
-    return o.bq == 32 && steps <= 8 && (m + o.bq - 1) / o.bq * ((n + o.bp - 1) / o.bp) <= compute_units();
+    return o.bq == 32 && steps <= 8 && tiles_of(o, m, n) <= compute_units();
 }
 
 // Whether c's rows leave with the streaming hint.  Rows on whole lines of memory do (bf16 2048^3 9.1 -> 8.5 us, 16384x4096x4096 127.8 -> 125.4).  Of others two
@@ -70,9 +74,8 @@ struct Launch {
         const Form &o = kForms[form];
         p.tiles_p = (p.n + o.bp - 1) / o.bp;
         p.tiles_q = (p.m + o.bq - 1) / o.bq;
-        const int64_t tiles = (int64_t)p.tiles_p * p.tiles_q;
-        if (tiles > 0x7FFFFFFFll) return fail(AGH_ERANGE, "%s: %d x %d: too many tiles", name, p.m, p.n);
-        blocks = (unsigned)tiles;
+        if (!launches(o, p.m, p.n)) return fail(AGH_ERANGE, "%s: a result of %d x %d: too many tiles", name, p.m, p.n);
+        blocks = (unsigned)(p.tiles_p * p.tiles_q);
         return AGH_OK;
     }
     template <bool RAW, int TP, int TQ, int WK, int U>
@@ -125,7 +128,8 @@ int gemm_entry(const char *name, int64_t m, int64_t k, int64_t n, const void *a_
     }
     const int64_t steps = steps_of(k);
     Launch<T> l = {name, {(const unsigned char *)a_codes, (const unsigned char *)a_scales, (const unsigned char *)b_codes, (const unsigned char *)b_scales,
-                          (T *)c + off_c, rsc, csc, bias ? (const T *)bias + off_bias : nullptr, bias_stride, (int)m, (int)n, (int)steps, act, rows_stream<T>((T *)c + off_c, rsc, m, n), 0, 0}, nullptr, 0, 0};
+                          (T *)c + off_c, rsc, csc, bias ? (const T *)bias + off_bias : nullptr, bias_stride, (int)m, (int)n, (int)steps, act,
+                          rows_stream<T>((T *)c + off_c, rsc, m, n), 0, 0}, nullptr, 0, 0};
     return l.run(choose_form(m, n, steps, sizeof(T)));
 }
 

@@ -184,12 +184,8 @@ int check_quantized(const char *name, const void *codes, const void *scales) {
     if (((uintptr_t)codes & 15) || ((uintptr_t)scales & 3)) return fail(AGH_EINVAL, "%s: codes must be 16-byte and scales 4-byte aligned", name);
     return AGH_OK;
 }
-int waves_grid(const char *name, int64_t items, unsigned &blocks) {
-    const int64_t n = (items + kThreads / 64 - 1) / (kThreads / 64);
-    if (n > 0x7FFFFFFFll) return fail(AGH_ERANGE, "%s: too many blocks", name);
-    blocks = (unsigned)n;
-    return AGH_OK;
-}
+// workgroups of four waves; sizes_fit keeps them below 2^24
+unsigned waves_grid(int64_t items) { return (unsigned)((items + kThreads / 64 - 1) / (kThreads / 64)); }
 
 template <typename T>
 int quantize_entry(const char *name, const void *x, int64_t off, int64_t rs, int64_t cs, int64_t rows, int64_t k, void *codes, void *scales) {
@@ -211,8 +207,7 @@ int dequantize_entry(const char *name, const void *codes, const void *scales, in
     const unsigned char *c = (const unsigned char *)codes, *s = (const unsigned char *)scales;
     T *to = (T *)y + off;
     const int64_t items = cs == 1 ? (rows + 15) / 16 * steps : (rows + 63) / 64 * steps * 4;
-    unsigned blocks;
-    if (int rc = waves_grid(name, items, blocks)) return rc;
+    const unsigned blocks = waves_grid(items);
     if (cs == 1)
         hipLaunchKernelGGL(dequantize_rows_kernel<T>, dim3(blocks), dim3(kThreads), 0, stream(), c, s, (int)rows, (int)k, steps, items, to, rs,
                            ((uintptr_t)to | (uint64_t)rs * sizeof(T)) % 128 == 0);
@@ -230,31 +225,24 @@ namespace mx {
 template <typename T>
 int quantize_launch(const char *name, const T *x, int64_t rs, int64_t cs, int64_t rows, int64_t k, void *codes, void *scales) {
     const int steps = (int)steps_of(k);
-    unsigned blocks;
     if (cs == 1) {
         const int64_t frags = (rows + 15) / 16 * steps;
-        if (int rc = waves_grid(name, frags, blocks)) return rc;
-        hipLaunchKernelGGL(quantize_rows_kernel<T>, dim3(blocks), dim3(kThreads), 0, stream(), x, rs, (int)rows, (int)k, steps, frags,
+        hipLaunchKernelGGL(quantize_rows_kernel<T>, dim3(waves_grid(frags)), dim3(kThreads), 0, stream(), x, rs, (int)rows, (int)k, steps, frags,
                            (unsigned char *)codes, (unsigned char *)scales);
         AGH_LAUNCH_CHECK(name);
         return AGH_OK;
     }
     if constexpr (sizeof(T) == 2) {
         if (rs == 1 && rows >= 16) {
-            const int64_t tiles = (rows + 63) / 64 * steps;
-            if (tiles > 0x7FFFFFFFll) return fail(AGH_ERANGE, "%s: too many blocks", name);
-            hipLaunchKernelGGL(quantize_columns_kernel, dim3((unsigned)tiles), dim3(kThreads), 0, stream(), x, cs, (int)rows, (int)k, steps, (unsigned char *)codes,
+            hipLaunchKernelGGL(quantize_columns_kernel, dim3((unsigned)((rows + 63) / 64 * steps)), dim3(kThreads), 0, stream(), x, cs, (int)rows, (int)k, steps, (unsigned char *)codes,
                                (unsigned char *)scales);
             AGH_LAUNCH_CHECK(name);
             return AGH_OK;
         }
     }
-    {
-        const int64_t items = (rows + 63) / 64 * steps * 4;
-        if (int rc = waves_grid(name, items, blocks)) return rc;
-        hipLaunchKernelGGL(quantize_strided_kernel<T>, dim3(blocks), dim3(kThreads), 0, stream(), x, rs, cs, (int)rows, (int)k, steps, items,
-                           (unsigned char *)codes, (unsigned char *)scales);
-    }
+    const int64_t items = (rows + 63) / 64 * steps * 4;
+    hipLaunchKernelGGL(quantize_strided_kernel<T>, dim3(waves_grid(items)), dim3(kThreads), 0, stream(), x, rs, cs, (int)rows, (int)k, steps, items, (unsigned char *)codes,
+                       (unsigned char *)scales);
     AGH_LAUNCH_CHECK(name);
     return AGH_OK;
 }

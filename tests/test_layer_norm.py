@@ -157,6 +157,59 @@ def test_layer_norm_many_wide_rows(ag, dtype, rows, cols):
 
 
 @gpu
+def test_more_columns_than_a_launch_adds_at_once(ag):
+    """2^20 groups of 16 columns and some: the workgroups that add the shares of dw and db take a second turn."""
+    rng = np.random.default_rng(3)
+    cols = 2**24 + 1000
+    x, w, b, dy = make(rng, 1, cols, "bf16")
+    layer = ag.LayerNorm(ag.Tensor.from_array(w[0]), ag.Tensor.from_array(b[0]))
+    tx, tdy = ag.Tensor.from_array(x[0]), ag.Tensor.from_array(dy[0])
+    y, mean, rstd = layer.forward_train(tx)
+    _, dw, db = (values_of(t) for t in layer.backward(tx, tdy, mean, rstd))
+    h = (x[1] - values_of(mean)[:, None]) * values_of(rstd)[:, None]
+    # one row: dy * h in f32 (three roundings) and one to bf16
+    want = (dy[1] * h)[0]
+    assert np.all(np.abs(dw - want) <= np.abs(want) * (2.0**-8 + 2.0**-21) + 1e-38) and np.array_equal(db, dy[1][0])
+    assert np.all(np.abs(values_of(y) - (h * w[1] + b[1])) <= 2.0**-8 * 1.01 * np.abs(h * w[1] + b[1]) + 2.0**-20 * (np.abs(h * w[1]) + np.abs(b[1])))
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols", [(140000, 16384), (70000, 32776)])
+def test_rows_beyond_32_bits(ag, rows, cols):
+    """4.6 GB of bf16, in rows that a workgroup holds and longer ones: rows behind 4 GiB are found, in both directions and in place.  The rows repeat with a
+    period of 8, and a row's results depend on the row alone."""
+    from autograph_amd._ffi import check
+    rng = np.random.default_rng(5)
+    x, w, b, dy = make(rng, 8, cols, "bf16")
+    layer = ag.LayerNorm(ag.Tensor.from_array(w[0]), ag.Tensor.from_array(b[0]))
+    few, few_dy = ag.Tensor.from_array(x[0]), ag.Tensor.from_array(dy[0])
+    y, mean, rstd = layer.forward_train(few)
+    dx = layer.backward(few, few_dy, mean, rstd)[0]
+
+    def many(t):
+        out, have = ag.Tensor.uninit((rows, cols), "bf16"), 8
+        check(ag.lib.agh_memcpy_d2d(out.buffer.ptr, t.buffer.ptr, 8 * cols * 2))
+        while have < rows:
+            n = min(have, rows - have)
+            check(ag.lib.agh_memcpy_d2d(out.buffer.ptr + have * cols * 2, out.buffer.ptr, n * cols * 2))
+            have += n
+        return out
+    mx, mdy = many(few), many(few_dy)
+    my, mmean, mrstd = layer.forward_train(mx)
+    mdx, dw, db = layer.backward(mx, mdy, mmean, mrstd)
+    tail = lambda t: t.slice_rows(rows - 8, rows).into_array()  # noqa: E731
+    assert np.array_equal(tail(my), y.into_array()) and np.array_equal(mmean.into_array()[-8:], mean.into_array())
+    assert np.array_equal(tail(mdx), dx.into_array()) and np.array_equal(tail(mx), x[0])
+    # dw, db: 8750 or 17500 times the sum of 8 rows; a chain of f32 sums is shorter than 2000, and one rounding to bf16
+    h = (x[1] - values_of(mean)[:, None]) * values_of(rstd)[:, None]
+    for got, terms in ((dw, dy[1] * h), (db, dy[1])):
+        want, size = terms.sum(0) * (rows // 8), np.abs(terms).sum(0) * (rows // 8)
+        assert np.all(np.abs(values_of(got) - want) <= 2.0**-8 * 1.01 * np.abs(want) + 2000 * 2.0**-24 * size)
+    check(ag.lib.agh_layer_norm_bf16(mx.buffer.ptr, layer.weight.buffer.ptr, layer.bias.buffer.ptr, EPS, mx.buffer.ptr, None, None, rows, cols))
+    assert np.array_equal(tail(mx), y.into_array())
+
+
+@gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_without_weight_or_bias(ag, dtype):
     rng = np.random.default_rng(5)

@@ -82,6 +82,15 @@ def test_buffer_sizes():
     assert MxTensor
 
 
+def test_sizes_that_a_launch_cannot_count():
+    """2^24 pieces of 64 rows x 128 values, a workgroup of 256 each, are the first that do not fit (64 x (2^31 - 513) is 2^24 - 4 of
+    them); refused before memory is asked for."""
+    from autograph_amd import _ffi
+    a, b = C.c_size_t(), C.c_size_t()
+    for rows, k, code in ((2**30 - 64, 128, 0), (2**30 - 63, 128, -4), (2**30, 128, -4), (64, 2**31 - 513, 0), (65, 2**31 - 513, -4), (64 * 4095, 128 * 4096, 0), (64 * 4096, 128 * 4096, -4)):
+        assert _ffi.lib.agh_mxfp4_bytes(rows, k, C.byref(a), C.byref(b)) == code, (rows, k)
+
+
 @pytest.mark.parametrize("rows,k", [(1, 1), (16, 128), (70, 300), (130, 33)])
 def test_places_do_not_overlap(rows, k):
     from autograph_amd import MxTensor
