@@ -72,7 +72,7 @@ int agh_free(void *ptr);
 int agh_cache_release(void);
 /* Bytes and blocks held for reuse, blocks currently handed out (any pointer may be null). */
 int agh_cache_stats(size_t *cached_bytes, size_t *cached_blocks, size_t *live_blocks);
-/* Bytes of the library's own workspace (split-K partials, reordered filter banks; both streams' blocks) and the number of
+/* Bytes of the library's own workspace (split-K partials, reordered filter banks, quantised inputs; both streams' blocks) and the number of
  * outgrown workspace blocks kept alive for live graphs.  None of this memory is the caller's; the figures let a caller
  * that must not allocate verify that a call sequence did not grow it. */
 int agh_workspace_stats(size_t *workspace_bytes, size_t *retired_blocks);
@@ -428,7 +428,7 @@ int agh_layer_norm_bf16(const void *x, const void *weight, const void *bias, flo
  *   dx = rstd * (g - sum g / cols - h * sum (g * h) / cols), dweight = sum over rows of dy * h, dbias = sum over rows of dy
  * x, dy, dx: [rows, cols] in standard layout, dx may be x or dy; mean, rstd: as the forward call wrote them.  Each of dx, dweight
  * and dbias may be null and is then not formed.  Sums are f32 and added in an order that depends on the sizes alone, results
- * rounded once.  rows == 0 writes zeros to dweight and dbias.  Uses the library's workspace. */
+ * rounded once.  rows == 0 writes zeros to dweight and dbias.  Uses the library's workspace for dweight and dbias. */
 int agh_layer_norm_backward_f32(const void *x, const void *dy, const void *weight, const void *mean, const void *rstd,
                                 void *dx, void *dweight, void *dbias, int64_t rows, int64_t cols);
 int agh_layer_norm_backward_bf16(const void *x, const void *dy, const void *weight, const void *mean, const void *rstd,
@@ -445,7 +445,8 @@ int agh_layer_norm_backward_bf16(const void *x, const void *dy, const void *weig
  *           ((r / 16 * steps + b / 4) * 64 + b % 4 * 16 + r % 16) * 16, steps = ceil(k / 128)
  *   scales  4-byte aligned: their byte is at ((r / 64 * steps + b / 4) * 64 + b % 4 * 16 + r % 16) * 4 + r / 16 % 4
  * Values behind k are zeros: codes 0, and the scale byte 0 where a whole block lies behind k; the last 128 of a row are always whole.
- * Rows behind the last one (r up to a multiple of 16, of 64 for the scales) may hold anything. */
+ * Rows behind the last one (r up to a multiple of 16, of 64 for the scales) may hold anything.  rows and k are below 2^31 - 512, and
+ * ceil(rows / 64) * steps below 2^24 (69 GB of codes), else AGH_ERANGE. */
 int agh_mxfp4_bytes(int64_t rows, int64_t k, size_t *codes, size_t *scales);
 
 /* x [rows, k] with element strides rs, cs (any; blocks run along k, so the transposed view of a matrix quantises it along its columns):
@@ -464,8 +465,7 @@ int agh_dequantize_mxfp4_bf16(const void *codes, const void *scales, int64_t row
 
 /* c[off_c + i*rsc + j*csc] = act(sum_x a[i][x] * b[j][x] + bias[off_bias + j*bias_stride]), i < m, j < n: a [m, k] and b [n, k] quantised, both
  * along k.  Sums are f32 on the matrix cores, bias (may be null) and act are applied in f32 and the result is rounded once.  c must not overlap
- * the operands and its elements must be distinct addresses; m, n or k == 0 is allowed (k == 0 yields act(bias)).  May use the library's
- * workspace. */
+ * the operands and its elements must be distinct addresses; m, n or k == 0 is allowed (k == 0 yields act(bias)).  No workspace. */
 int agh_gemm_mxfp4_f32(int64_t m, int64_t k, int64_t n, const void *a_codes, const void *a_scales, const void *b_codes,
                        const void *b_scales, void *c, int64_t off_c, int64_t rsc, int64_t csc,
                        const void *bias, int64_t off_bias, int64_t bias_stride, int act);
@@ -475,7 +475,8 @@ int agh_gemm_mxfp4_bf16(int64_t m, int64_t k, int64_t n, const void *a_codes, co
 
 /* Dense forward with a quantised weight: x [m, k] (element strides rsx, csx) is quantised along k as agh_quantize_mxfp4_<T> does and multiplied with
  * w, the weight [k, n] quantised along k (n rows of k values, as agh_quantize_mxfp4_<T> writes them from the transposed view).  The same bits as
- * the two calls.  Uses the library's workspace. */
+ * the two calls.  c must not overlap x.  The quantised input lies in the library's workspace, or with few rows in registers: run a call that is to be
+ * captured once eagerly, as for a product with split-K. */
 int agh_dense_mxfp4_f32(int64_t m, int64_t k, int64_t n, const void *x, int64_t off_x, int64_t rsx, int64_t csx,
                         const void *w_codes, const void *w_scales, void *c, int64_t off_c, int64_t rsc, int64_t csc,
                         const void *bias, int64_t off_bias, int64_t bias_stride, int act);
