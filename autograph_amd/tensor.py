@@ -105,9 +105,12 @@ def _dims(shape):
 
 
 def _std_strides(shape):
-    if len(shape) == 2:
+    axes = len(shape)
+    if axes == 2:
         return (shape[1], 1)
-    if len(shape) == 4:
+    if axes == 1:
+        return (1,)
+    if axes == 4:
         _, c, h, w = shape
         return (c * h * w, h * w, w, 1)
     strides, acc = [], 1
@@ -404,13 +407,10 @@ class Tensor:
 
     # -- layer norm over the last axis (no counterpart in the reference) --
     def _norm_vector(self, v, name):
-        """The address of a weight or bias of layer norm, checked, and what keeps it alive until the call."""
-        if v is None:
-            return None, None
+        """A weight or bias of layer norm, checked, in standard layout."""
         if v.dtype != self.dtype or v.shape != self.shape[-1:]:
             raise AghError(-1, f"layer_norm: {name} must be a {self.dtype} vector of length {self.shape[-1]}")
-        v = v.as_standard_layout()
-        return v._data_ptr(), v
+        return v if v.strides == (1,) else v.as_standard_layout()
 
     def layer_norm(self, weight=None, bias=None, epsilon=1e-5, stats=False):
         """(x - mean) / sqrt(var + epsilon) * weight + bias over the last axis.  With `stats`: (y, mean, rstd), the f32 tensors that
@@ -419,15 +419,21 @@ class Tensor:
         if not shape:
             raise AghError(-1, "layer_norm: a tensor without axes")
         x = self.as_standard_layout()
-        w, _w = self._norm_vector(weight, "weight")
-        b, _b = self._norm_vector(bias, "bias")
+        w = b = None  # (what they hold lives until the call has been issued)
+        if weight is not None:
+            weight = self._norm_vector(weight, "weight")
+            w = weight._data_ptr()
+        if bias is not None:
+            bias = self._norm_vector(bias, "bias")
+            b = bias._data_ptr()
         y = _uninit(shape, dtype)
         call = calls.agh_layer_norm_f32 if dtype == F32 else calls.agh_layer_norm_bf16
-        rows = shape[0] if len(shape) == 2 else math.prod(shape[:-1])
+        lead = shape[:-1]
+        rows = shape[0] if len(shape) == 2 else math.prod(lead)
         if not stats:
             call(x._data_ptr(), w, b, epsilon, y.buffer.ptr, None, None, rows, shape[-1])
             return y
-        mean, rstd = _uninit(shape[:-1], F32), _uninit(shape[:-1], F32)
+        mean, rstd = _uninit(lead, F32), _uninit(lead, F32)
         call(x._data_ptr(), w, b, epsilon, y.buffer.ptr, mean.buffer.ptr, rstd.buffer.ptr, rows, shape[-1])
         return y, mean, rstd
 
@@ -443,12 +449,15 @@ class Tensor:
         if mean.dtype != F32 or rstd.dtype != F32 or mean.shape != lead or rstd.shape != lead:
             raise AghError(-1, f"layer_norm_backward: mean and rstd must be f32 tensors of {lead}, found {mean.dtype} {mean.shape}, {rstd.dtype} {rstd.shape}")
         x, dy, mean, rstd = self.as_standard_layout(), output_grad.as_standard_layout(), mean.as_standard_layout(), rstd.as_standard_layout()
-        w, _w = self._norm_vector(weight, "weight")
-        dx = _uninit(shape, dtype)
-        dw, db = (None, None) if weight is None else (_uninit(shape[-1:], dtype), _uninit(shape[-1:], dtype))
+        rows = shape[0] if len(shape) == 2 else math.prod(lead)
         call = calls.agh_layer_norm_backward_f32 if dtype == F32 else calls.agh_layer_norm_backward_bf16
-        call(x._data_ptr(), dy._data_ptr(), w, mean._data_ptr(), rstd._data_ptr(), dx.buffer.ptr, None if dw is None else dw.buffer.ptr,
-             None if db is None else db.buffer.ptr, shape[0] if len(shape) == 2 else math.prod(lead), shape[-1])
+        if weight is None:
+            dx = _uninit(shape, dtype)
+            call(x._data_ptr(), dy._data_ptr(), None, mean._data_ptr(), rstd._data_ptr(), dx.buffer.ptr, None, None, rows, shape[-1])
+            return dx, None, None
+        weight = self._norm_vector(weight, "weight")
+        dx, dw, db = _uninit(shape, dtype), _uninit(weight.shape, dtype), _uninit(weight.shape, dtype)
+        call(x._data_ptr(), dy._data_ptr(), weight._data_ptr(), mean._data_ptr(), rstd._data_ptr(), dx.buffer.ptr, dw.buffer.ptr, db.buffer.ptr, rows, shape[-1])
         return dx, dw, db
 
     # -- MXFP4 (no counterpart in the reference) --
