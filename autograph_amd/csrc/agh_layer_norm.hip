@@ -261,31 +261,34 @@ __global__ __launch_bounds__(THREADS, THREADS == 512 && VPT == 2 ? 4 : 1) void l
     }
 }
 
-// dw (blockIdx.y 0) and db out of n workgroups' shares: a workgroup adds 16 columns at a time, 4 threads of 4 columns by 64 parts of the shares
+// dw (blockIdx.y 0) and db out of n workgroups' shares: a workgroup adds kAddColumns columns at a time, a line of memory of each share, a thread 4 columns of every
+// kAddParts-th share.  (16 columns, half a line, by 64 threads: with the pass before bf16 16384x4096 77.2 us against 75.1, 2048x2048 15.7 against 14.6; 32 by 32: 65536x84
+// 17.9 against 16.6.)
+constexpr int kAddWorkgroup = 1024, kAddColumns = 32, kAddThreads = kAddColumns / 4, kAddParts = kAddWorkgroup / kAddThreads;
 template <typename T>
-__global__ __launch_bounds__(kThreads) void add_shares_kernel(const float *__restrict__ shares, int n, int pitch, T *__restrict__ dw, T *__restrict__ db, int cols) {
-    __shared__ f32x4_t part[kThreads / 64][4];
-    const int c = threadIdx.x & 3, p = threadIdx.x >> 2;
+__global__ __launch_bounds__(kAddWorkgroup) void add_shares_kernel(const float *__restrict__ shares, int n, int pitch, T *__restrict__ dw, T *__restrict__ db, int cols) {
+    __shared__ f32x4_t part[kAddWorkgroup / 64][kAddThreads];
+    const int c = threadIdx.x % kAddThreads, p = threadIdx.x / kAddThreads;
     T *out = blockIdx.y ? db : dw;
     if (!out) return;
-    for (int64_t col = (int64_t)blockIdx.x * 16 + c * 4; col - c * 4 < cols; col += (int64_t)gridDim.x * 16) {
+    for (int64_t col = (int64_t)blockIdx.x * kAddColumns + c * 4; col - c * 4 < cols; col += (int64_t)gridDim.x * kAddColumns) {
         f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
         if (col < cols) {
             const float *from = shares + blockIdx.y * (int64_t)pitch + col;
 #pragma unroll 8
-            for (int i = p; i < n; i += 64) s += *(const f32x4_t *)(from + (int64_t)i * 2 * pitch);
+            for (int i = p; i < n; i += kAddParts) s += *(const f32x4_t *)(from + (int64_t)i * 2 * pitch);
         }
 #pragma unroll
-        for (int d = 4; d < 64; d *= 2)
+        for (int d = kAddThreads; d < 64; d *= 2)
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[i] += __shfl_xor(s[i], d);
         __syncthreads();  // the turn before has been read
-        if ((threadIdx.x & 63) < 4) part[threadIdx.x >> 6][c] = s;
+        if ((threadIdx.x & 63) < kAddThreads) part[threadIdx.x >> 6][c] = s;
         __syncthreads();
-        if (threadIdx.x >= 4 || col >= cols) continue;
+        if (threadIdx.x >= kAddThreads || col >= cols) continue;
         s = part[0][c];
 #pragma unroll
-        for (int i = 1; i < kThreads / 64; ++i) s += part[i][c];
+        for (int i = 1; i < kAddWorkgroup / 64; ++i) s += part[i][c];
         for (int i = 0; i < 4 && col + i < cols; ++i) out[col + i] = Elem<T>::from_f32(s[i]);
     }
 }
@@ -477,8 +480,8 @@ struct Backward {
     int cols, pitch;
 
     int add(const float *shares, int64_t n) const {
-        const int64_t wgs = ((int64_t)cols + 15) / 16;
-        hipLaunchKernelGGL(add_shares_kernel<T>, dim3((unsigned)(wgs < kMostWorkgroups ? wgs : kMostWorkgroups), 2), dim3(kThreads), 0, stream(), shares, (int)n, pitch, dw, db, cols);
+        const int64_t wgs = ((int64_t)cols + kAddColumns - 1) / kAddColumns;
+        hipLaunchKernelGGL(add_shares_kernel<T>, dim3((unsigned)(wgs < kMostWorkgroups ? wgs : kMostWorkgroups), 2), dim3(kAddWorkgroup), 0, stream(), shares, (int)n, pitch, dw, db, cols);
         AGH_LAUNCH_CHECK(name);
         return AGH_OK;
     }
@@ -489,7 +492,8 @@ struct Backward {
         // 16384x4096, 512 threads: 256 workgroups 98.5 us, 512 76.6, 1024 87.7; 4096x16384: 256 89.8, 512 97.7), and two turns each at least.
         // Where a quarter of the threads has no columns, a third fills the gap (512 threads by 1, f32 21845x1536 86.2 -> 78.5, bf16 13107x2560 55.6 -> 53.1; all at work, 8192x4096 bf16 46.2 -> 47.4).
         const bool gaps = cols <= TPR * VPT * Group<T>::VE / 4 * 3;
-        const int64_t turns = (rows + per_wg - 1) / per_wg, most = (int64_t)compute_units() * (TPR <= 64 ? VPT <= 2 ? 3 : 2 : TPR == 512 && VPT <= 2 ? VPT == 1 && gaps ? 3 : 2 : 1);
+        constexpr int each = TPR <= 64 ? (VPT <= 2 ? 3 : 2) : TPR == 512 && VPT <= 2 ? 2 : 1;
+        const int64_t turns = (rows + per_wg - 1) / per_wg, most = (int64_t)compute_units() * (TPR == 512 && VPT == 1 && gaps ? 3 : each);
         int64_t wgs = THREADS == 1024 && TPR <= 64 ? 1 : (turns + 1) / 2;
         if (wgs > most) wgs = most;
         float *shares = nullptr;

@@ -158,9 +158,9 @@ def test_layer_norm_many_wide_rows(ag, dtype, rows, cols):
 
 @gpu
 def test_more_columns_than_a_launch_adds_at_once(ag):
-    """2^20 groups of 16 columns and some: the workgroups that add the shares of dw and db take a second turn."""
+    """2^20 groups of 32 columns and some: the workgroups that add the shares of dw and db take a second turn."""
     rng = np.random.default_rng(3)
-    cols = 2**24 + 1000
+    cols = 2**25 + 1000
     x, w, b, dy = make(rng, 1, cols, "bf16")
     layer = ag.LayerNorm(ag.Tensor.from_array(w[0]), ag.Tensor.from_array(b[0]))
     tx, tdy = ag.Tensor.from_array(x[0]), ag.Tensor.from_array(dy[0])
