@@ -5,9 +5,9 @@
 // All sums are f32, whatever the element type, and every result is rounded to it once.
 //
 // Bounded by memory: each element is read once and written once.  A row stays in the registers of the threads that share it, in 16-byte
-// groups, between its sums and its result; so the squares can be taken of deviations from the finished mean.  Up to 8 groups a lane a row belongs to
+// groups, between its sums and its result; so the squares can be taken of deviations from the finished mean.  Up to 4 groups a lane a row belongs to
 // one wave, whose sums need neither LDS nor a barrier, longer ones to a workgroup.  Threads keep their columns from row to row: weight and bias are read
-// once, and the backward pass adds its columns' shares of dw and db in registers.
+// once, and the backward pass adds its columns' shares of dw and db in registers.  bf16 16384x4096: 47.8 us forward (5.6 TB/s), 75 to 81 backward (5.0 to 5.4).
 #include "agh_groups.h"
 
 using namespace agh;

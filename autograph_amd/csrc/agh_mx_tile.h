@@ -5,6 +5,10 @@
 // and each LDS read 16 bytes a lane in order: no bank conflicts, no address arithmetic beyond a scalar addition a load.
 // A wave holds two sets of fragments: while step s is multiplied out of one, the reads of step s + 1 go into the other, spread over the MFMAs (all
 // at once they would ask the LDS for twice what it gives).  Behind the barrier early in step s, the stage that step s was read from is refilled.
+//
+// 8192^3 with 256x256 tiles, 8 waves: 222 us, 4.9 PFLOP/s, 73 % of a loop of nothing but these instructions on such codes.  A step reads 96 KB of LDS and writes 32 KB, 1024
+// cycles, as long as its instructions take; left out for timing, one operand's reads give 203 us, the loads 189, both operands' reads and the loads 149.  Four waves
+// of 128x128, with a third less to read, have no second wave to hide what they wait for: 289.
 #pragma once
 #include "agh_gemm_kernel.h"
 #include "agh_mx.h"
