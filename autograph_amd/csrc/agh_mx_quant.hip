@@ -3,7 +3,7 @@
 //   s = clamp(floor(log2 max |v|) - 2, -127, 127) over a block of 32, code = E2M1(v / 2^s) rounded half to even, magnitudes above 6 to 6.
 // A block with an infinity or a NaN gets the scale byte 255 and stands for 32 NaNs: E2M1 has neither, and clipping would hide them.
 // Bounded by memory: bf16 16384x4096 27 us along the rows (6.3 TB/s), its inverse 25 (6.8).
-// The conversion instruction divides by 2^s, rounds and saturates; its results were compared with the formula's at every border between codes, for every s.
+// The conversion instruction divides by 2^s, rounds and saturates; its results are compared with the formula's at every border between codes, under scales from the smallest to the largest.
 #include "agh_mx_quant.h"
 
 using namespace agh;
