@@ -15,24 +15,34 @@ namespace {
 // `tile` (half as much again for f32 results of the large tiles, which they are bound by) + `step` for every 128 of k, but at least `least` (fetching the kernel's code,
 // storing the result).  Over 520 products, sizes drawn at random, both types, no operand in a cache from the call before, the form chosen takes 1.02 of the best one's
 // time in the mean, and more than 1.12 of it in 4 of 100.  (128x128 tiles with k split between two halves of a workgroup took 11.5 instead of 12.4 us at 2048x4096x1000
-// and lost where k is short; not taken.)
+// and lost where k is short; 64x64 tiles, straight from memory, are never the best of these. Neither is taken.)
 struct Form {
     int bp, bq, threads;
     double start, tile, step, least;
 };
 constexpr Form kForms[] = {{16, 16, 512, 2.5, 0.2, 0.034, 0.4},   {32, 16, 512, 2.5, 0.2, 0.064, 0.5},   {16, 32, 512, 3.1, 0.13, 0.042, 0.73},
-                           {32, 32, 256, 2.5, 0.2, 0.071, 0.48},  {32, 64, 256, 3.6, 0.65, 0.077, 1.25}, {64, 64, 256, 3.2, 2.66, 0.174, 2.7},
-                           {128, 128, 256, 4.0, 1.6, 0.19, 0.0},  {256, 256, 512, 2.8, 5.9, 0.54, 0.0}};
+                           {32, 32, 256, 2.5, 0.2, 0.071, 0.48},  {32, 64, 256, 3.6, 0.65, 0.077, 1.25}, {128, 128, 256, 4.0, 1.6, 0.19, 0.0},
+                           {256, 256, 512, 2.8, 5.9, 0.54, 0.0}};
 constexpr int kFormCount = sizeof(kForms) / sizeof(kForms[0]);
 int64_t tiles_of(const Form &o, int64_t m, int64_t n) { return ((n + o.bp - 1) / o.bp) * ((m + o.bq - 1) / o.bq); }
 bool launches(const Form &o, int64_t m, int64_t n) { return tiles_of(o, m, n) <= 0xFFFFFFFFll / o.threads; }  // a launch counts its work items in 32 bits
 
+// Whether Dense's input is quantised in the product's launch, by every workgroup again, instead of by a launch of its own (2.5 to 2.9 us, and as much of the host's time):
+// up to 16 rows always (1x4096x4096 4.6 us against 3.7 + 2.5, 16x4096x4096 6.6 against 3.7 + 2.5), to about 500 where no CU has a second tile and k is short (64x256x256 3.5
+// against 2.8 + 2.9, 100x1000x300 4.8 against 2.8 + 2.8; 200x2000x100 6.8 against 3.0 + 2.8, 64x4096x4096 11.3 against 5.4 + 2.7).
+bool quantises_itself(const Form &o, int64_t m, int64_t n, int64_t steps) {
+    if (o.bq == 16) return true;
+    return o.bp == 32 && o.bq == 32 && steps <= 8 && tiles_of(o, m, n) <= compute_units();
+}
+
+// The same for Dense as for the product, whose bits it gives.
 int choose_form(int64_t m, int64_t n, int64_t steps, size_t element) {
     int best = kFormCount - 1;
     double least = 1e30;
     for (int f = 0; f < kFormCount; ++f) {
         const Form &o = kForms[f];
-        if ((o.bq == 16 && m > 16) || !launches(o, m, n)) continue;
+        // (up to 16 rows: the 32 of the others would be half empty, and Dense would need a second launch)
+        if ((o.bp < 128 && (o.bq == 16) != (m <= 16)) || !launches(o, m, n)) continue;
         const double tiles = (double)tiles_of(o, m, n), cus = compute_units();
         // the tiled kernels' workgroups fill a CU, one or two at a time; many small ones share it evenly
         const bool large = o.bp >= 128;
@@ -41,15 +51,6 @@ int choose_form(int64_t m, int64_t n, int64_t steps, size_t element) {
         if (us < least) least = us, best = f;
     }
     return best;
-}
-
-// Whether Dense's input is quantised in the product's launch, by every workgroup again, instead of by a launch of its own (2.5 to 2.9 us, and as much of the host's time):
-// up to 16 rows always (1x4096x4096 4.6 us against 3.7 + 2.5, 16x4096x4096 6.6 against 3.7 + 2.5), to about 500 where no CU has a second tile and k is short (64x256x256 3.5
-// against 2.8 + 2.9, 100x1000x300 4.8 against 2.8 + 2.8; 200x2000x100 6.8 against 3.0 + 2.8, 64x4096x4096 11.3 against 5.4 + 2.7).
-bool quantises_itself(int form, int64_t m, int64_t n, int64_t steps) {
-    const Form &o = kForms[form];
-    if (o.bq == 16) return true;
-    return o.bq == 32 && steps <= 8 && tiles_of(o, m, n) <= compute_units();
 }
 
 // Whether c's rows leave with the streaming hint.  Rows on whole lines of memory do (bf16 2048^3 9.1 -> 8.5 us, 16384x4096x4096 127.8 -> 125.4).  Of others two
@@ -88,11 +89,10 @@ struct Launch {
         switch (form) {
             case 0: x ? direct<true, 1, 1, 8, 2>(blocks) : direct<false, 1, 1, 8, 4>(blocks); break;
             case 1: x ? direct<true, 2, 1, 8, 2>(blocks) : direct<false, 2, 1, 8, 4>(blocks); break;
-            case 2: x ? direct<true, 1, 2, 8, 1>(blocks) : direct<false, 1, 2, 8, 4>(blocks); break;
+            case 2: direct<false, 1, 2, 8, 4>(blocks); break;
             case 3: x ? direct<true, 2, 2, 4, 1>(blocks) : direct<false, 2, 2, 4, 2>(blocks); break;
             case 4: direct<false, 2, 4, 4, 2>(blocks); break;
-            case 5: direct<false, 4, 4, 4, 2>(blocks); break;
-            case 6: hipLaunchKernelGGL((mx_tile_kernel<T, 128, 128, 2, 2, 4>), dim3(blocks), dim3(256), 0, stream(), p); break;
+            case 5: hipLaunchKernelGGL((mx_tile_kernel<T, 128, 128, 2, 2, 4>), dim3(blocks), dim3(256), 0, stream(), p); break;
             default: hipLaunchKernelGGL((mx_tile_kernel<T, 256, 256, 4, 2, 4>), dim3(blocks), dim3(512), 0, stream(), p); break;
         }
         AGH_LAUNCH_CHECK(name);
@@ -144,7 +144,7 @@ int dense_entry(const char *name, int64_t m, int64_t k, int64_t n, const void *x
         if (int rc = check_operand(name, "w", w_codes, w_scales)) return rc;
         const int64_t steps = steps_of(k);
         const int form = choose_form(m, n, steps, sizeof(T));
-        if (csx == 1 && quantises_itself(form, m, n, steps)) {
+        if (csx == 1 && quantises_itself(kForms[form], m, n, steps)) {
             // few rows: quantised by every workgroup for itself, in one launch
             Launch<T> l = {name, {nullptr, nullptr, (const unsigned char *)w_codes, (const unsigned char *)w_scales, (T *)c + off_c, rsc, csc,
                                   bias ? (const T *)bias + off_bias : nullptr, bias_stride, (int)m, (int)n, (int)steps, act, false, 0, 0}, (const T *)x + off_x, rsx, (int)k};

@@ -282,6 +282,15 @@ def test_dot(ag, dtype, m, n, k):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,n,k", [(9, 7703, 1100), (16, 20001, 130), (1, 20001, 70), (45, 709, 3111), (300, 2390, 2500), (1000, 2900, 300), (4132, 1193, 47), (1813, 6715, 60),
+                                   (4183, 3204, 894)])
+def test_dot_every_tile(ag, dtype, m, n, k):
+    """Sizes for which the wider tiles are chosen, in order 32x16, 16x32, 32x64, 128x128 and 256x256, ragged in every direction."""
+    test_dot(ag, dtype, m, n, k)
+
+
+@gpu
 def test_dot_is_exact_where_f32_is(ag):
     """Integers as codes: every sum below 2^24, so every result equals the integer product, whatever the order."""
     rng = np.random.default_rng(8)
@@ -341,6 +350,13 @@ def test_strided_output_and_bias(ag, dtype, m, n, k):
         rest = np.ones(got.size, bool)
         rest[at.ravel()] = False
         assert (got[rest] == 7).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,n,k", [(300, 2390, 2500), (1000, 2900, 300), (1813, 6715, 60), (1813, 6720, 60)])
+def test_strided_output_of_wide_tiles(ag, dtype, m, n, k):
+    test_strided_output_and_bias(ag, dtype, m, n, k)
 
 
 @gpu
