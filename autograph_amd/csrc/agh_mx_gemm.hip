@@ -27,12 +27,14 @@ constexpr int kFormCount = sizeof(kForms) / sizeof(kForms[0]);
 int64_t tiles_of(const Form &o, int64_t m, int64_t n) { return ((n + o.bp - 1) / o.bp) * ((m + o.bq - 1) / o.bq); }
 bool launches(const Form &o, int64_t m, int64_t n) { return tiles_of(o, m, n) <= 0xFFFFFFFFll / o.threads; }  // a launch counts its work items in 32 bits
 
-// Whether Dense's input is quantised in the product's launch, by every workgroup again, instead of by a launch of its own (2.5 to 2.9 us, and as much of the host's time):
-// up to 16 rows always (1x4096x4096 4.6 us against 3.7 + 2.5, 16x4096x4096 6.6 against 3.7 + 2.5), to about 500 where no CU has a second tile and k is short (64x256x256 3.5
-// against 2.8 + 2.9, 100x1000x300 4.8 against 2.8 + 2.8; 200x2000x100 6.8 against 3.0 + 2.8, 64x4096x4096 11.3 against 5.4 + 2.7).
-bool quantises_itself(const Form &o, int64_t m, int64_t n, int64_t steps) {
-    if (o.bq == 16) return true;
-    return o.bp == 32 && o.bq == 32 && steps <= 8 && tiles_of(o, m, n) <= compute_units();
+// Whether Dense's input is quantised in the product's launch, by every workgroup again, instead of by a launch of its own, about 3 us and as much of the host's time.  What it
+// costs a CU for every 128 of k, fitted in us to the difference: the conversion, and its rows' bytes at 50 bytes a ns (one launch / two, bf16: 1x4096x4096 4.6 / 6.2 us, 64x256x256
+// 3.5 / 5.7, 100x1000x300 4.8 / 5.6, 16x4096x32000 23.3 / 16.0, 200x2000x100 6.8 / 5.8; f32: 1x4096x32000 17.9 / 16.0, 16x4096x32000 40 / 17.2).
+bool quantises_itself(const Form &o, int64_t m, int64_t n, int64_t steps, size_t element) {
+    if (o.bq != 16 && !(o.bp == 32 && o.bq == 32)) return false;
+    const double tiles = (double)tiles_of(o, m, n), cus = compute_units(), turns = tiles > cus ? tiles / cus : 1.0;
+    const double bytes = (double)((m < o.bq ? m : o.bq) * kStep * (int64_t)element);
+    return turns * (double)steps * ((element == 4 ? 0.037 : 0.02) + bytes * 2e-5) < 3.2;
 }
 
 // The same for Dense as for the product, whose bits it gives.
@@ -144,7 +146,7 @@ int dense_entry(const char *name, int64_t m, int64_t k, int64_t n, const void *x
         if (int rc = check_operand(name, "w", w_codes, w_scales)) return rc;
         const int64_t steps = steps_of(k);
         const int form = choose_form(m, n, steps, sizeof(T));
-        if (csx == 1 && quantises_itself(kForms[form], m, n, steps)) {
+        if (csx == 1 && quantises_itself(kForms[form], m, n, steps, sizeof(T))) {
             // few rows: quantised by every workgroup for itself, in one launch
             Launch<T> l = {name, {nullptr, nullptr, (const unsigned char *)w_codes, (const unsigned char *)w_scales, (T *)c + off_c, rsc, csc,
                                   bias ? (const T *)bias + off_bias : nullptr, bias_stride, (int)m, (int)n, (int)steps, act, false, 0, 0}, (const T *)x + off_x, rsx, (int)k};
