@@ -537,9 +537,9 @@ int backward_entry(const char *name, const void *x, const void *dy, const void *
     // as the forward pass, but 512 threads beyond 256 groups: a thread's columns take their sums' registers too (16384x4096: bf16, 512 groups, a wave with 8 each
     // 111 us, 256 threads with 2 79.7, 512 with 1 76.6; f32, 1024 groups, 512 with 2 145.6, 1024 with 1 147)
     // short rows and few turns of 1024 threads: one workgroup, which needs no second launch (f32, us against two: 100x84 7.8 / 11.7, 128x84 9.4 / 10.3, 256x60 5.9 / 10.3; 256x84
-    // 16.2 / 10.3, 512x60 9.1 / 8.3)
+    // 16.2 / 10.3, 512x60 9.1 / 8.3; bf16, called without pause, where two launches take 7.5: 64x512 8.3, 128x512 13.1, 256x128 8.1)
     if (groups <= 16 && rows <= 256) return f.template run<1024, 16, 1>();
-    if (groups <= 64 && rows <= 128) return f.template run<1024, 64, 1>();
+    if (groups <= 64 && rows <= (VE == 8 ? 64 : 128)) return f.template run<1024, 64, 1>();
     if (groups <= 16) return f.template run<256, 16, 1>();
     if (groups <= 64) return f.template run<256, 64, 1>();
     if (groups <= 128) return f.template run<256, 64, 2>();
@@ -549,7 +549,8 @@ int backward_entry(const char *name, const void *x, const void *dy, const void *
     // (bf16 4096x8192: 512 threads with 2 in 135 registers, one workgroup a unit, 62.8 us; in 128, two, 53.0; 1024 threads 49.9.  5461x6144: 62.2, 53.7, 52.9; 7281x4608: 71.7, 55.6, 60.5.
     // f32 8192x4096: 512 threads 69.3, 1024 76.7)
     if (groups <= (VE == 8 ? 768 : 1024)) return f.template run<512, 512, 2>();
-    if (groups <= 1024) return f.template run<1024, 1024, 1>();
+    if constexpr (VE == 8)
+        if (groups <= 1024) return f.template run<1024, 1024, 1>();
     if (groups <= 1536) return f.template run<512, 512, 3>();
     if (groups <= 2048) return f.template run<512, 512, 4>();
     // (bf16 has twice the sums for each group, which leaves the compiler no registers: 1638x20480 190 us against 74 when the rows are read again)

@@ -127,7 +127,7 @@ def test_the_oracle():
 # ---- on the GPU ----
 
 SHAPES = [(1, 1), (1, 4096), (3, 2), (7, 16), (5, 31), (100, 84), (33, 129), (64, 512), (19, 1000), (9, 1001), (6, 2048), (5, 2047), (4, 4097), (3, 8192), (2, 12345),
-          (2, 16384), (3, 20000), (2, 70000), (1000, 10), (2500, 64), (1500, 257)]
+          (2, 16384), (3, 20000), (2, 70000), (1000, 10), (2500, 64), (1500, 257), (333, 700)]
 
 
 @gpu
