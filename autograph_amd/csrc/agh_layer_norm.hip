@@ -262,12 +262,13 @@ __global__ __launch_bounds__(THREADS, THREADS == 512 && VPT == 2 ? 4 : 1) void l
 }
 
 // dw (blockIdx.y 0) and db out of n workgroups' shares: a workgroup adds kAddColumns columns at a time, a line of memory of each share, a thread 4 columns of every
-// kAddParts-th share.  (16 columns, half a line, by 64 threads: with the pass before bf16 16384x4096 77.2 us against 75.1, 2048x2048 15.7 against 14.6; 32 by 32: 65536x84
+// PARTS-th share.  (16 columns, half a line, by 64 threads: with the pass before bf16 16384x4096 77.2 us against 75.1, 2048x2048 15.7 against 14.6; 32 by 32: 65536x84
 // 17.9 against 16.6.)
-constexpr int kAddWorkgroup = 1024, kAddColumns = 32, kAddThreads = kAddColumns / 4, kAddParts = kAddWorkgroup / kAddThreads;
-template <typename T>
-__global__ __launch_bounds__(kAddWorkgroup) void add_shares_kernel(const float *__restrict__ shares, int n, int pitch, T *__restrict__ dw, T *__restrict__ db, int cols) {
-    __shared__ f32x4_t part[kAddWorkgroup / 64][kAddThreads];
+constexpr int kAddColumns = 32, kAddThreads = kAddColumns / 4;
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void add_shares_kernel(const float *__restrict__ shares, int n, int pitch, T *__restrict__ dw, T *__restrict__ db, int cols) {
+    constexpr int PARTS = THREADS / kAddThreads;
+    __shared__ f32x4_t part[THREADS / 64][kAddThreads];
     const int c = threadIdx.x % kAddThreads, p = threadIdx.x / kAddThreads;
     T *out = blockIdx.y ? db : dw;
     if (!out) return;
@@ -276,7 +277,7 @@ __global__ __launch_bounds__(kAddWorkgroup) void add_shares_kernel(const float *
         if (col < cols) {
             const float *from = shares + blockIdx.y * (int64_t)pitch + col;
 #pragma unroll 8
-            for (int i = p; i < n; i += kAddParts) s += *(const f32x4_t *)(from + (int64_t)i * 2 * pitch);
+            for (int i = p; i < n; i += PARTS) s += *(const f32x4_t *)(from + (int64_t)i * 2 * pitch);
         }
 #pragma unroll
         for (int d = kAddThreads; d < 64; d *= 2)
@@ -288,7 +289,7 @@ __global__ __launch_bounds__(kAddWorkgroup) void add_shares_kernel(const float *
         if (threadIdx.x >= kAddThreads || col >= cols) continue;
         s = part[0][c];
 #pragma unroll
-        for (int i = 1; i < kAddWorkgroup / 64; ++i) s += part[i][c];
+        for (int i = 1; i < THREADS / 64; ++i) s += part[i][c];
         for (int i = 0; i < 4 && col + i < cols; ++i) out[col + i] = Elem<T>::from_f32(s[i]);
     }
 }
@@ -481,7 +482,10 @@ struct Backward {
 
     int add(const float *shares, int64_t n) const {
         const int64_t wgs = ((int64_t)cols + kAddColumns - 1) / kAddColumns;
-        hipLaunchKernelGGL(add_shares_kernel<T>, dim3((unsigned)(wgs < kMostWorkgroups ? wgs : kMostWorkgroups), 2), dim3(kAddWorkgroup), 0, stream(), shares, (int)n, pitch, dw, db, cols);
+        const dim3 grid((unsigned)(wgs < kMostWorkgroups ? wgs : kMostWorkgroups), 2);
+        // (few shares of many columns: smaller workgroups, more of them side by side; with the pass before bf16 16x16384 11.9 us, by 1024 threads 15.5)
+        if (n <= 64) hipLaunchKernelGGL((add_shares_kernel<T, 256>), grid, dim3(256), 0, stream(), shares, (int)n, pitch, dw, db, cols);
+        else hipLaunchKernelGGL((add_shares_kernel<T, 1024>), grid, dim3(1024), 0, stream(), shares, (int)n, pitch, dw, db, cols);
         AGH_LAUNCH_CHECK(name);
         return AGH_OK;
     }
