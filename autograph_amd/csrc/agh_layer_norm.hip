@@ -168,6 +168,11 @@ __global__ __launch_bounds__(wg_threads(TPR)) void layer_norm_kernel(const T *x,
     }
 }
 
+// rstd as the factor of the deviations.  Behind a row's end x is 0 and h = -mean rstd, which has to be finite: 0 * inf would be a NaN in all of dx.  It is, unless all the
+// row's values are one: else some value deviates from the mean by half a step of it, and rstd is at most 2^25 sqrt(C) / |mean|.  The deviations of a row of one value are 0,
+// and so is h whatever the factor is.  (Places behind the end left out, by a branch or a select for each group: 2 to 10 % of the time.)
+__device__ __forceinline__ float deviations_rstd(float mean, float rstd) { return __builtin_isinf(mean * rstd) && !__builtin_isinf(rstd) ? 0.0f : rstd; }
+
 // Backward: dx, and this workgroup's shares of dw and db.  shares [gridDim.x][2][pitch]: f32, or with one workgroup nothing, then dw and db are written here.
 template <typename T, int THREADS, int TPR, int VPT>
 __global__ __launch_bounds__(THREADS, THREADS == 512 && VPT == 2 ? 4 : 1) void layer_norm_backward_kernel(
@@ -193,15 +198,15 @@ __global__ __launch_bounds__(THREADS, THREADS == 512 && VPT == 2 ? 4 : 1) void l
             xv[j] = load_row<T, (VPT > 3 && TPR > 64)>(x + row * cols, e, cols);
             gv[j] = load_row<T, (VPT > 3 && TPR > 64)>(dy + row * cols, e, cols);
         }
-        const float mean = mean_in[row], rstd = rstd_in[row];
+        const float mean = mean_in[row], rstd = rstd_in[row], rstd_h = deviations_rstd(mean, rstd);
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             keep_packed(wv[j]);
 #pragma unroll
             for (int i = 0; i < VE; ++i) {
-                // (behind the row's end dy is 0 and so is every term, or a NaN where the whole row is NaN)
-                const float d = G::get(gv[j], i), h = (G::get(xv[j], i) - mean) * rstd, g = d * G::get(wv[j], i);
+                // (behind the row's end dy is 0 and so is every term, or a NaN where the whole row is NaN: h is finite there)
+                const float d = G::get(gv[j], i), h = (G::get(xv[j], i) - mean) * rstd_h, g = d * G::get(wv[j], i);
                 ab[j][i] += d;
                 aw[j][i] += d * h;
                 s[0] += g;
@@ -211,7 +216,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 512 && VPT == 2 ? 4 : 1) void l
         if (dx) {
             row_sums<TPR>(s, part + (TPR > 64 ? turn * 2 * (THREADS / 64) + sub * (TPR / 64) * 2 : 0));
             turn ^= 1;
-                s[0] *= per;
+            s[0] *= per;
             s[1] *= per;
 #pragma unroll
             for (int j = 0; j < VPT; ++j) {
@@ -222,7 +227,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 512 && VPT == 2 ? 4 : 1) void l
                 keep_packed(wv[j]);
 #pragma unroll
                 for (int i = 0; i < VE; ++i) {
-                    const float d = G::get(gv[j], i), h = (G::get(xv[j], i) - mean) * rstd, g = d * G::get(wv[j], i);
+                    const float d = G::get(gv[j], i), h = (G::get(xv[j], i) - mean) * rstd_h, g = d * G::get(wv[j], i);
                     f[i] = rstd * (g - s[0] - h * s[1]);
                 }
                 if (e < cols) store_group(dx + row * cols, e, cols, G::pack(f));
@@ -362,7 +367,7 @@ __global__ __launch_bounds__(kLongThreads) void layer_norm_backward_long_kernel(
     __shared__ float part[kLongThreads / 64];
     const float per = 1.0f / (float)cols;
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-        const float mean = mean_in[row], rstd = rstd_in[row];
+        const float mean = mean_in[row], rstd = rstd_in[row], rstd_h = deviations_rstd(mean, rstd);
         const T *xr = x + row * cols, *dyr = dy + row * cols;
         T *dxr = dx + row * cols;
         float sg = 0.0f, sgh = 0.0f;
@@ -373,7 +378,7 @@ __global__ __launch_bounds__(kLongThreads) void layer_norm_backward_long_kernel(
             for (int i = 0; i < VE; ++i) {  // (behind the row's end dy is 0)
                 const float g = G::get(gv, i) * G::get(wv, i);
                 sg += g;
-                sgh += g * ((G::get(xv, i) - mean) * rstd);
+                sgh += g * ((G::get(xv, i) - mean) * rstd_h);
             }
         }
         sg = workgroup_sum(sg, part) * per;
@@ -383,7 +388,7 @@ __global__ __launch_bounds__(kLongThreads) void layer_norm_backward_long_kernel(
             const u32x4_t xv = G::load(xr, e, cols), gv = G::load(dyr, e, cols), wv = load_or(w, e, cols, 1.0f);
             float f[VE];
 #pragma unroll
-            for (int i = 0; i < VE; ++i) f[i] = rstd * (G::get(gv, i) * G::get(wv, i) - sg - (G::get(xv, i) - mean) * rstd * sgh);
+            for (int i = 0; i < VE; ++i) f[i] = rstd * (G::get(gv, i) * G::get(wv, i) - sg - (G::get(xv, i) - mean) * rstd_h * sgh);
             store_group(dxr, e, cols, G::pack(f));
         }
     }
