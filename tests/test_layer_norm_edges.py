@@ -23,3 +23,47 @@ def test_gradients_of_rows_far_from_zero(ag, dtype, rows, cols):  # noqa: F811
     got = [values_of(t) for t in tx.layer_norm_backward(tdy, tw, tm, tr)]
     assert np.isfinite(got[0]).all()
     check_backward(got, x[1], dy[1], w[1], mean.astype(np.float64), rstd.astype(np.float64), dtype)
+
+
+COLS = [1, 3, 10, 100, 193, 1000, 1001, 3001, 5003, 7001, 12345, 16384, 20001, 40003]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("cols", COLS)
+def test_rows_of_one_value(ag, dtype, cols):  # noqa: F811
+    """Their mean is that value: y is the bias, exactly, and rstd 1 / sqrt(eps) within three roundings.  A first mean off by at most L u |x| (L as in
+    test_layer_norm.py) leaves deviations that are all the same, and their mean, off by L u of itself, the rest of it: less than half a step for L^2 u < 1/2, L < 2896."""
+    rng = np.random.default_rng(22)
+    x = as_type(np.repeat(np.array([[1000.1], [-7.3e5], [0.1], [3.0], [-1e4], [0.0], [2.0**20 + 0.1], [-65000.7], [1e-30], [1e15]]), cols, 1), dtype)
+    _, w, b, _ = make(rng, 1, cols, dtype)
+    tx, tw, tb = (ag.Tensor.from_array(v) for v in (x[0], w[0], b[0]))
+    y, mean, rstd = tx.layer_norm(tw, tb, EPS, stats=True)
+    assert np.array_equal(values_of(mean), x[1][:, 0])
+    assert np.all(np.abs(values_of(rstd) - EPS**-0.5) <= 4 * U * EPS**-0.5)
+    assert np.array_equal(values_of(y), np.repeat(b[1][None, :], len(x[1]), 0))
+    # with eps 0 the formula divides 0 by 0, in those rows alone
+    mixed = x[0].copy()
+    mixed[4:8] = as_type(rng.standard_normal((4, cols)), dtype)[0]
+    mixed = ag.Tensor.from_array(mixed)
+    got, want = values_of(mixed.layer_norm(tw, tb, 0.0)), values_of(mixed.layer_norm(tw, tb, 1e-30))
+    one = [0, 1, 2, 3, 8, 9] if cols > 1 else list(range(10))
+    assert np.isnan(got[one]).all()
+    rest = [r for r in range(10) if r not in one]
+    assert np.array_equal(got[rest], want[rest]) and np.isfinite(got[rest]).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("cols", COLS[2:])
+def test_mean_of_rows_far_from_zero(ag, dtype, cols):  # noqa: F811
+    """Where the spread is small against the mean, the mean is the rounded one: off by u |mean| and by the f32 sum of the deviations from a first one, (L + 3) u mean |d|,
+    |d| larger than the true deviation by at most the first mean's L u mean |x|."""
+    rng = np.random.default_rng(23)
+    spread = np.array([[1.0], [20.0], [0.01], [5.0], [1e-3], [40.0], [2.0], [0.3]])
+    x = as_type(1000 + spread * rng.standard_normal((8, cols)), dtype)
+    mean = values_of(ag.Tensor.from_array(x[0]).layer_norm(stats=True)[1])
+    m = x[1].mean(1)
+    L = cols / 16 + 16
+    d = np.abs(x[1] - m[:, None]).mean(1) + L * U * np.abs(x[1]).mean(1)
+    assert np.all(np.abs(mean - m) <= U * np.abs(m) + (L + 3) * U * d)
