@@ -224,8 +224,8 @@ class LayerNorm:
         return x.layer_norm(self.weight, self.bias, self.epsilon, stats=True)
 
     def backward(self, x, output_grad, mean, rstd):
-        """(dx, dweight, dbias)."""
-        return x.layer_norm_backward(output_grad, self.weight, mean, rstd)
+        """(dx, dweight, dbias), None for a parameter that the layer has not."""
+        return x.layer_norm_backward(output_grad, self.weight, mean, rstd, bias=self.bias is not None)
 
 
 class MaxPool2:

@@ -437,9 +437,9 @@ class Tensor:
         call(x._data_ptr(), w, b, epsilon, y.buffer.ptr, mean.buffer.ptr, rstd.buffer.ptr, rows, shape[-1])
         return y, mean, rstd
 
-    def layer_norm_backward(self, output_grad, weight, mean, rstd):
-        """Gradients (dx, dweight, dbias) of `self.layer_norm(weight, bias, stats=True)`, `self` being its input; with weight None
-        (dx, None, None)."""
+    def layer_norm_backward(self, output_grad, weight, mean, rstd, bias=None):
+        """Gradients (dx, dweight, dbias) of `self.layer_norm(weight, .., stats=True)`, `self` being its input.  With weight None dweight is None; dbias is
+        formed where `bias` is true, by default where there is a weight, and else None."""
         shape, dtype = self.shape, self.dtype
         if not shape:
             raise AghError(-1, "layer_norm_backward: a tensor without axes")
@@ -451,13 +451,16 @@ class Tensor:
         x, dy, mean, rstd = self.as_standard_layout(), output_grad.as_standard_layout(), mean.as_standard_layout(), rstd.as_standard_layout()
         rows = shape[0] if len(shape) == 2 else math.prod(lead)
         call = calls.agh_layer_norm_backward_f32 if dtype == F32 else calls.agh_layer_norm_backward_bf16
-        if weight is None:
-            dx = _uninit(shape, dtype)
-            call(x._data_ptr(), dy._data_ptr(), None, mean._data_ptr(), rstd._data_ptr(), dx.buffer.ptr, None, None, rows, shape[-1])
-            return dx, None, None
-        weight = self._norm_vector(weight, "weight")
-        dx, dw, db = _uninit(shape, dtype), _uninit(weight.shape, dtype), _uninit(weight.shape, dtype)
-        call(x._data_ptr(), dy._data_ptr(), weight._data_ptr(), mean._data_ptr(), rstd._data_ptr(), dx.buffer.ptr, dw.buffer.ptr, db.buffer.ptr, rows, shape[-1])
+        dx, dw, db = _uninit(shape, dtype), None, None
+        w = dw_ptr = db_ptr = None  # (what they hold lives until the call has been issued)
+        if weight is not None:
+            weight = self._norm_vector(weight, "weight")
+            dw = _uninit(shape[-1:], dtype)
+            w, dw_ptr = weight._data_ptr(), dw.buffer.ptr
+        if weight is not None if bias is None else bias:
+            db = _uninit(shape[-1:], dtype)
+            db_ptr = db.buffer.ptr
+        call(x._data_ptr(), dy._data_ptr(), w, mean._data_ptr(), rstd._data_ptr(), dx.buffer.ptr, dw_ptr, db_ptr, rows, shape[-1])
         return dx, dw, db
 
     # -- MXFP4 (no counterpart in the reference) --

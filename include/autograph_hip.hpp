@@ -356,7 +356,11 @@ public:
     // with the f32 statistics, one value a row, that layer_norm_backward takes
     LayerNormed<T> layer_norm_train(const Tensor *weight, const Tensor *bias, float epsilon = 1e-5f) const;
     // gradients with respect to *this (the input), weight and bias
-    LayerNormGrads<T> layer_norm_backward(const Tensor &output_grad, const Tensor &weight, const Tensor<float> &mean, const Tensor<float> &rstd) const;
+    LayerNormGrads<T> layer_norm_backward(const Tensor &output_grad, const Tensor &weight, const Tensor<float> &mean, const Tensor<float> &rstd) const {
+        return layer_norm_backward(output_grad, &weight, mean, rstd, true);
+    }
+    // where the weight may be null; the bias gradient if it is asked for.  A gradient that is not formed has length 0.
+    LayerNormGrads<T> layer_norm_backward(const Tensor &output_grad, const Tensor *weight, const Tensor<float> &mean, const Tensor<float> &rstd, bool bias) const;
 
     // -- MXFP4 (no counterpart in the reference): blocks of 32 along `axis`, the one a product will sum over --
     MxTensor quantize_mxfp4(int axis = 1) const;
@@ -429,18 +433,18 @@ template <typename T> LayerNormed<T> Tensor<T>::layer_norm_train(const Tensor *w
     return out;
 }
 template <typename T>
-LayerNormGrads<T> Tensor<T>::layer_norm_backward(const Tensor &output_grad, const Tensor &weight, const Tensor<float> &mean, const Tensor<float> &rstd) const {
+LayerNormGrads<T> Tensor<T>::layer_norm_backward(const Tensor &output_grad, const Tensor *weight, const Tensor<float> &mean, const Tensor<float> &rstd, bool bias) const {
     if (dim_.empty()) bail("layer_norm_backward: a tensor without axes");
-    const Shape lead(dim_.begin(), dim_.end() - 1), features{dim_.back()};
+    const Shape lead(dim_.begin(), dim_.end() - 1), features{dim_.back()}, none{0};
     if (output_grad.dim_ != dim_) bail("layer_norm_backward: expected a gradient of " + shape_str(dim_) + ", found " + shape_str(output_grad.dim_));
     if (mean.shape() != lead || rstd.shape() != lead) bail("layer_norm_backward: mean and rstd must be " + shape_str(lead));
-    check_features(weight, "weight");
-    const Tensor x = as_standard_layout(), dy = output_grad.as_standard_layout(), w = weight.as_standard_layout();
+    if (weight) check_features(*weight, "weight");
+    const Tensor x = as_standard_layout(), dy = output_grad.as_standard_layout(), w = weight ? weight->as_standard_layout() : Tensor();
     const Tensor<float> m = mean.as_standard_layout(), r = rstd.as_standard_layout();
-    LayerNormGrads<T> out{uninit(dim_), uninit(features), uninit(features)};
-    check((kBf16 ? agh_layer_norm_backward_bf16 : agh_layer_norm_backward_f32)(x.data_ptr(), dy.data_ptr(), w.data_ptr(), m.data_ptr(), r.data_ptr(),
-                                                                               out.input.buffer_ptr(), out.weight.buffer_ptr(), out.bias.buffer_ptr(),
-                                                                               shape_len(lead), dim_.back()));
+    LayerNormGrads<T> out{uninit(dim_), uninit(weight ? features : none), uninit(bias ? features : none)};
+    check((kBf16 ? agh_layer_norm_backward_bf16 : agh_layer_norm_backward_f32)(
+        x.data_ptr(), dy.data_ptr(), weight ? w.data_ptr() : nullptr, m.data_ptr(), r.data_ptr(), out.input.buffer_ptr(), weight ? out.weight.buffer_ptr() : nullptr,
+        bias ? out.bias.buffer_ptr() : nullptr, shape_len(lead), dim_.back()));
     return out;
 }
 
@@ -568,6 +572,10 @@ template <typename T> struct LayerNorm {
     float epsilon = 1e-5f;
     Tensor<T> forward(const Tensor<T> &input) const { return input.layer_norm(weight.get(), bias.get(), epsilon); }
     LayerNormed<T> forward_train(const Tensor<T> &input) const { return input.layer_norm_train(weight.get(), bias.get(), epsilon); }
+    // a gradient for each parameter that the layer has, of length 0 for the other
+    LayerNormGrads<T> backward(const Tensor<T> &input, const Tensor<T> &output_grad, const Tensor<float> &mean, const Tensor<float> &rstd) const {
+        return input.layer_norm_backward(output_grad, weight.get(), mean, rstd, bias != nullptr);
+    }
 };
 // `MaxPool2` (layer.rs:1149-1216); the stride defaults to the filter (layer.rs:535-539)
 template <typename T> struct MaxPool2 {
