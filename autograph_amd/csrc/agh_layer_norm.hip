@@ -438,10 +438,11 @@ __global__ __launch_bounds__(kLongThreads) void layer_norm_backward_long_kernel(
     }
 }
 
-// a thread a group of columns, a share for every gridDim.y-th row
+// a thread a group of columns, a share for every gridDim.y-th row; without shares (one for all rows) the results themselves
 template <typename T>
 __global__ __launch_bounds__(kThreads) void column_shares_kernel(const T *__restrict__ x, const T *__restrict__ dy, const float *__restrict__ mean,
-                                                                 const float *__restrict__ rstd, float *__restrict__ shares, int64_t rows, int cols, int pitch) {
+                                                                 const float *__restrict__ rstd, float *__restrict__ shares, T *__restrict__ dw, T *__restrict__ db,
+                                                                 int64_t rows, int cols, int pitch) {
     using G = Group<T>;
     constexpr int VE = G::VE;
     const int64_t e = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * VE;
@@ -457,6 +458,11 @@ __global__ __launch_bounds__(kThreads) void column_shares_kernel(const T *__rest
             sb[i] += g;
             sw[i] += g * ((G::get(xv, i) - m) * s);
         }
+    }
+    if (!shares) {
+        if (dw) store_group(dw, (int)e, cols, G::pack(sw));
+        if (db) store_group(db, (int)e, cols, G::pack(sb));
+        return;
     }
     float *mine = shares + (int64_t)blockIdx.y * 2 * pitch + e;  // pitch: whole groups
 #pragma unroll
@@ -559,13 +565,18 @@ struct Backward {
     }
     int run_long() const {
         if (dw || db) {  // (before dx, which may overwrite x or dy)
-            const int64_t n = rows < 16 ? rows : rows / 16 < 64 ? rows / 16 : 64;
-            float *shares;
-            if (int rc = workspace((size_t)n * 2 * pitch * sizeof(float), (void **)&shares)) return rc;
-            hipLaunchKernelGGL(column_shares_kernel<T>, dim3((unsigned)((pitch / Group<T>::VE + kThreads - 1) / kThreads), (unsigned)n), dim3(kThreads), 0, stream(), x, dy, mean, rstd,
-                               shares, rows, cols, pitch);
+            // Shares of 16 rows, and no more of them than the workgroups that keep the chip busy: their memory, which the library keeps, stays below 34 MB however long a row is.
+            // Where the columns alone are workgroups enough, one share, which is the result.
+            const int64_t groups = pitch / Group<T>::VE, wgs = (groups + kThreads - 1) / kThreads, most = (int64_t)compute_units() * 8 / wgs;
+            int64_t n = rows < 16 ? rows : rows / 16 < 64 ? rows / 16 : 64;
+            if (n > most) n = most > 1 ? most : 1;
+            float *shares = nullptr;
+            if (n > 1)
+                if (int rc = workspace((size_t)n * 2 * pitch * sizeof(float), (void **)&shares)) return rc;
+            hipLaunchKernelGGL(column_shares_kernel<T>, dim3((unsigned)wgs, (unsigned)n), dim3(kThreads), 0, stream(), x, dy, mean, rstd, shares, dw, db, rows, cols, pitch);
             AGH_LAUNCH_CHECK(name);
-            if (int rc = add(shares, n)) return rc;
+            if (shares)
+                if (int rc = add(shares, n)) return rc;
         }
         if (dx) {
             hipLaunchKernelGGL(layer_norm_backward_long_kernel<T>, dim3((unsigned)(rows < kMostWorkgroups ? rows : kMostWorkgroups)), dim3(kLongThreads), 0, stream(), x, dy, w,

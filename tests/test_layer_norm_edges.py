@@ -67,3 +67,40 @@ def test_mean_of_rows_far_from_zero(ag, dtype, cols):  # noqa: F811
     L = cols / 16 + 16
     d = np.abs(x[1] - m[:, None]).mean(1) + L * U * np.abs(x[1]).mean(1)
     assert np.all(np.abs(mean - m) <= U * np.abs(m) + (L + 3) * U * d)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,rows,cols", [("bf16", 15, 2**22 + 8), ("f32", 15, 2**20 + 3), ("f32", 40, 2**21), ("bf16", 600, 70001)])
+def test_scratch_of_long_rows(ag, dtype, rows, cols):  # noqa: F811
+    """The library's own memory for the weight gradients does not grow with the rows (8 bytes for each element of 15 rows, 503 MB, were kept).  The values are ones that
+    f32 sums hold exactly: mean 0, rstd 1, x and dy small integers, so dw and db are whole numbers."""
+    import ctypes as C
+    check = ag._ffi.check
+    rng = np.random.default_rng(24)
+    x, dy = (as_type(np.tile(rng.integers(-2, 3, (rows, 4099)), (1, -(-cols // 4099)))[:, :cols], dtype) for _ in range(2))
+    tx, tdy, tw = ag.Tensor.from_array(x[0]), ag.Tensor.from_array(dy[0]), ag.Tensor.from_array(as_type(np.ones(cols), dtype)[0])
+    mean, rstd = ag.Tensor.from_array(np.zeros(rows, np.float32)), ag.Tensor.from_array(np.ones(rows, np.float32))
+    check(ag.lib.agh_sync())
+    check(ag.lib.agh_cache_release())
+    before, after = C.c_size_t(), C.c_size_t()
+    check(ag.lib.agh_workspace_stats(C.byref(before), None))
+    _, dw, db = tx.layer_norm_backward(tdy, tw, mean, rstd)
+    check(ag.lib.agh_workspace_stats(C.byref(after), None))
+    assert after.value - before.value <= 80 << 20  # at most 34 MB are asked for; the workspace grows by doubling
+    for got, want in ((dw, (x[1][:, :4099] * dy[1][:, :4099]).sum(0)), (db, dy[1][:, :4099].sum(0))):
+        want = as_type(want, dtype)[1]  # whole numbers below 2^24, rounded once
+        assert np.array_equal(values_of(got), np.tile(want, -(-cols // 4099))[:cols])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_no_rows_of_many_columns(ag, dtype):  # noqa: F811
+    """Zeros in every column, also behind the 2^25 that one launch adds at once."""
+    cols = 2**25 + 1000
+    s = ag.Tensor.zeros((0,), "f32")
+    x, w = ag.Tensor.zeros((0, cols), dtype), ag.Tensor.zeros((cols,), dtype)
+    out = [ag.Tensor.uninit((cols,), dtype) for _ in range(2)]
+    for t in out:
+        ag._ffi.check(ag.lib.agh_memset(t._ptr(), 0xFF, t.buffer.nbytes))
+    ag._ffi.check(getattr(ag.lib, f"agh_layer_norm_backward_{dtype}")(x._ptr(), x._ptr(), w._ptr(), s._ptr(), s._ptr(), None, out[0]._ptr(), out[1]._ptr(), 0, cols))
+    assert not any(t.into_array().any() for t in out)
