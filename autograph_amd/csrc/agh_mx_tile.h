@@ -28,8 +28,9 @@ struct Problem {
 };
 
 // Issued from inline assembly with the accumulator tied to the accumulation registers and updated in place: given the builtin, the register allocator
-// moves accumulators between the two register files inside the loop.  SP, SQ: which byte of the scale registers.  The same accumulator
-// is next touched a step later, so no result hazard arises between two of these.
+// moves accumulators between the two register files inside the loop.  SP, SQ: which byte of the scale registers.  Between two of these no wait is needed: an accumulator is C
+// and D in the same registers, and the hardware hands such a result on to the next instruction that adds to exactly those (the direct kernels do so back to back);
+// what it does not hand on, another overlap or a result as operand A or B, does not occur.
 template <int SP, int SQ>
 __device__ __forceinline__ void mfma(f32x4_t &c, u32x4_t p, u32x4_t q, uint32_t sp, uint32_t sq) {
     asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0] cbsz:4 blgp:4"
