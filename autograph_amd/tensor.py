@@ -501,7 +501,7 @@ class MxTensor:
         return MxTensor(self.codes, self.scales, self.shape[::-1], 1 - self.axis)
 
     def dequantize(self, dtype=F32):
-        """The values that the codes stand for; both types hold them exactly."""
+        """The values that the codes stand for; both types hold them exactly (from 2^128 on, under the scales 253 and 254 of `from_arrays`: infinities)."""
         if dtype not in _ITEMSIZE:
             raise AghError(-1, f"dequantize: unknown type {dtype!r}")
         y = _uninit(self.shape, dtype)

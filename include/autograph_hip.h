@@ -457,7 +457,7 @@ int agh_quantize_mxfp4_f32(const void *x, int64_t off_x, int64_t rs, int64_t cs,
 int agh_quantize_mxfp4_bf16(const void *x, int64_t off_x, int64_t rs, int64_t cs, int64_t rows, int64_t k, void *codes,
                             void *scales);
 /* The values that the codes stand for (exact in either type) into y [rows, k] with element strides rs, cs, whose elements must be
- * distinct addresses. */
+ * distinct addresses.  Under the scale bytes 253 and 254, which the quantiser above never writes, a code may stand for 2^128 or more: infinity. */
 int agh_dequantize_mxfp4_f32(const void *codes, const void *scales, int64_t rows, int64_t k, void *y, int64_t off_y,
                              int64_t rs, int64_t cs);
 int agh_dequantize_mxfp4_bf16(const void *codes, const void *scales, int64_t rows, int64_t k, void *y, int64_t off_y,
