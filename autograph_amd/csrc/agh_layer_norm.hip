@@ -600,10 +600,14 @@ int backward_entry(const char *name, const void *x, const void *dy, const void *
     if (rows == 0) return f.add(nullptr, 0);
     // as the forward pass, but 512 threads beyond 256 groups: a thread's columns take their sums' registers too (16384x4096: bf16, 512 groups, a wave with 8 each
     // 111 us, 256 threads with 2 79.7, 512 with 1 76.6; f32, 1024 groups, 512 with 2 145.6, 1024 with 1 147)
-    // short rows and few turns of 1024 threads: one workgroup, which needs no second launch (f32, us against two: 100x84 7.8 / 11.7, 128x84 9.4 / 10.3, 256x60 5.9 / 10.3; 256x84
-    // 16.2 / 10.3, 512x60 9.1 / 8.3; bf16, called without pause, where two launches take 7.5: 64x512 8.3, 128x512 13.1, 256x128 8.1)
-    if (groups <= 16 && rows <= 256) return f.template run<1024, 16, 1>();
-    if (groups <= 64 && rows <= (VE == 8 ? 64 : 128)) return f.template run<1024, 64, 1>();
+    // Few short rows: one workgroup of 1024 threads, which needs no second launch and, called after another from Python, saves 2 us of the host's time.  It is taken as far as such
+    // calls gain; replayed from a graph it loses before that.  us, one workgroup / two launches, in calls and in a graph: f32 64x84 7.2 / 9.4 and 6.1 / 5.7, 96x84 8.1 / 9.3 and 7.9 / 5.8,
+    // 128x84 9.7 / 9.4 and 9.6 / 5.9, 256x60 7.1 / 9.4 and 6.2 / 6.0, 512x60 9.6 / 9.3 and 9.5 / 6.0; bf16 32x512 7.3 / 9.2 and 6.1 / 5.8, 64x512 8.5 / 9.4 and 8.4 / 5.9, 96x512 11.0 / 9.3,
+    // 128x128 6.7 / 9.4 and 6.1 / 6.0, 192x84 8.5 / 9.2 and 8.3 / 7.0, 256x84 9.8 / 9.4.  So few that 256 threads are one workgroup too, and have
+    // one turn, bf16 up to two: those (in a graph f32 4x10 2.9 for 3.3, bf16 32x128 3.8 for 4.5; f32 with two turns 32x60 3.6 for 3.5).
+    constexpr int turns = VE == 8 ? 2 : 1;
+    if (groups <= 16 && rows > 16 * turns && rows <= (VE == 8 ? 192 : 256)) return f.template run<1024, 16, 1>();
+    if (groups > 16 && groups <= 64 && rows > 4 * turns && rows <= (VE == 8 ? 64 : 128)) return f.template run<1024, 64, 1>();
     if (groups <= 16) return f.template run<256, 16, 1>();
     if (groups <= 64) return f.template run<256, 64, 1>();
     if (groups <= 128) return f.template run<256, 64, 2>();

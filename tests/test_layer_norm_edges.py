@@ -104,3 +104,17 @@ def test_no_rows_of_many_columns(ag, dtype):  # noqa: F811
         ag._ffi.check(ag.lib.agh_memset(t._ptr(), 0xFF, t.buffer.nbytes))
     ag._ffi.check(getattr(ag.lib, f"agh_layer_norm_backward_{dtype}")(x._ptr(), x._ptr(), w._ptr(), s._ptr(), s._ptr(), None, out[0]._ptr(), out[1]._ptr(), 0, cols))
     assert not any(t.into_array().any() for t in out)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [4, 5, 8, 9, 16, 17, 32, 33, 64, 65, 128, 129, 192, 193, 256, 257])
+def test_gradients_of_few_rows(ag, dtype, rows):  # noqa: F811
+    """On both sides of the numbers of rows at which one workgroup takes over from several and gives way to them again."""
+    for cols in (30, 84, 200):
+        rng = np.random.default_rng(rows + cols)
+        x, w, _, dy = make(rng, rows, cols, dtype)
+        tx, tdy, tw = (ag.Tensor.from_array(v[0]) for v in (x, dy, w))
+        _, mean, rstd = tx.layer_norm(tw, stats=True)
+        got = [values_of(t) for t in tx.layer_norm_backward(tdy, tw, mean, rstd)]
+        check_backward(got, x[1], dy[1], w[1], values_of(mean), values_of(rstd), dtype)
