@@ -544,7 +544,7 @@ class MxTensor:
             check(lib.agh_memcpy_d2h(raw[-1].ctypes.data, b.ptr, b.nbytes))
         at_codes, at_scales = self._places(rows, k)
         packed = raw[0][at_codes[..., None] + np.arange(16)]
-        codes = np.stack((packed & 15, packed >> 4), -1).reshape(rows, -1)[:, :k]
+        codes = np.stack((packed & 15, packed >> 4), -1).reshape(rows, -(-k // 32) * 32)[:, :k]
         scales = raw[1][at_scales]
         return (codes, scales) if self.axis == 1 else (np.ascontiguousarray(codes.T), np.ascontiguousarray(scales.T))
 
@@ -560,8 +560,9 @@ class MxTensor:
         rows, k = codes.shape
         if scales.shape != (rows, -(-k // 32)) or (codes > 15).any():
             raise AghError(-1, f"MxTensor.from_arrays: codes below 16 and one scale for 32 of them expected, found {codes.shape} and {scales.shape}")
-        packed = np.zeros((rows, -(-k // 32), 32), np.uint8)
-        packed.reshape(rows, -1)[:, :k] = codes
+        packed = np.zeros((rows, -(-k // 32) * 32), np.uint8)
+        packed[:, :k] = codes
+        packed = packed.reshape(rows, -(-k // 32), 32)
         at_codes, at_scales = cls._places(rows, k)
         for b, at, values in ((out.codes, at_codes[..., None] + np.arange(16), packed[..., 0::2] | packed[..., 1::2] << 4), (out.scales, at_scales, scales)):
             raw = np.zeros(b.nbytes, np.uint8)

@@ -1,5 +1,7 @@
 """MXFP4 on inputs whose rows lie backwards, on top of each other or at odd places, in the launch that quantises its input itself and in the one before the
 product; and values at the end of f32."""
+import types
+
 import numpy as np
 import pytest
 
@@ -7,6 +9,18 @@ import mxfp4
 from test_mx import ag, as_type, check_product, values_of  # noqa: F401
 
 gpu = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("axis", [0, 1])
+@pytest.mark.parametrize("shape", [(0, 5), (5, 0), (0, 0), (0, 40), (40, 0)])
+def test_arrays_of_nothing(monkeypatch, shape, axis):
+    """A matrix without rows or columns has codes of its shape and scales for none of its blocks, both ways; without a device."""
+    from autograph_amd import MxTensor, tensor
+    monkeypatch.setattr(tensor, "Buffer", lambda nbytes: types.SimpleNamespace(ptr=0, nbytes=nbytes))
+    monkeypatch.setattr(tensor, "lib", types.SimpleNamespace(agh_memcpy_d2h=lambda *a: 0, agh_memcpy_h2d=lambda *a: 0, agh_sync=lambda: 0))
+    blocks = tuple(-(-n // 32) if a == axis else n for a, n in enumerate(shape))
+    assert tuple(a.shape for a in MxTensor.uninit(shape, axis).into_arrays()) == (shape, blocks)
+    assert MxTensor.from_arrays(np.zeros(shape, np.uint8), np.zeros(blocks, np.uint8), axis).shape == shape
 
 
 @gpu
