@@ -7,7 +7,7 @@
 // Bounded by memory: each element is read once and written once.  A row stays in the registers of the threads that share it, in 16-byte
 // groups, between its sums and its result; so the squares can be taken of deviations from the finished mean.  Up to 4 groups a lane a row belongs to
 // one wave, whose sums need neither LDS nor a barrier, longer ones to a workgroup.  Threads keep their columns from row to row: weight and bias are read
-// once, and the backward pass adds its columns' shares of dw and db in registers.  bf16 16384x4096: 47.8 us forward (5.6 TB/s), 75 to 81 backward (5.0 to 5.4).
+// once, and the backward pass adds its columns' shares of dw and db in registers.  bf16 16384x4096: 47.8 us forward (5.6 TB/s), 81 backward (5.0).
 #include "agh_groups.h"
 
 using namespace agh;
@@ -624,6 +624,7 @@ int backward_entry(const char *name, const void *x, const void *dy, const void *
     // (bf16 has twice the sums for each group, which leaves the compiler no registers: 1638x20480 190 us against 74 when the rows are read again)
     if constexpr (VE == 4) {
         if (groups <= 3 * 1024) return f.template run<1024, 1024, 3>();  // f32 3276x10240 85.7 us, 512 threads with 8 96
+        // (spills 40 registers, and is still the fastest of three by a wide margin: 4096x16384 178 us, 1024 threads with 4 224, read again 289; 4096x12292 141, 196, 217; one row 7.1, 10.7, 8.3)
         if (groups <= 4096) return f.template run<512, 512, 8>();
     }
     return f.run_long();

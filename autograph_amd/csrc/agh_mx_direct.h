@@ -1,7 +1,8 @@
 // MXFP4 product straight from memory, for results of few tiles: a workgroup's WK waves share one tile of 16 TP x 16 TQ and split k among themselves, so nothing that
 // one of them reads is of use to another, and fragments go from memory into the registers that the matrix instruction reads.  Their sums meet in LDS, added
 // in the waves' order.  With few rows of a (one token, a handful of requests) this is one pass over b: 1x4096x4096 with the
-// quantisation 4.6 us, 1.9 TB/s, bound by one wait for memory, the quantisation and the joining of the sums one behind the other.
+// quantisation 4.7 us, 1.9 TB/s.  A wave has 4 steps there and takes U = 2 at a time: two waits for memory, in each of which the second step's weights are requested
+// behind the first step's values of a, and then the quantisation and the joining of the sums, one behind the other.
 //
 // RAW: a is not quantised yet.  A lane quantises what its place in the fragment holds, 32 neighbours of one row, so the values never leave its
 // registers; every workgroup does it again, which for few rows is less than a launch of its own.
