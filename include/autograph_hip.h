@@ -417,7 +417,8 @@ int agh_relu_backward_bf16(const void *x, const void *dy, void *dx, int64_t n);
  * src/learn/neural_network/layer.rs:
  *   mean = sum x / cols, rstd = 1 / sqrt(sum (x - mean)^2 / cols + eps), y = (x - mean) * rstd * weight + bias
  * weight and bias have cols elements of the same type; a null weight stands for ones, a null bias for zeros.  mean and rstd,
- * rows floats each, are what the backward call takes; either may be null.  y may be x.  Sums are f32, y is rounded once.
+ * rows floats each, are what the backward call takes; either may be null.  y may be x.  Sums are f32, y is rounded once; a row of one
+ * value has that value as its mean, exactly (up to 2^21 columns).  Rows whose sum or whose squared deviations pass f32 (values from about 1e19 on) are out of range.
  * rows == 0 does nothing; cols must be at least 1, both below 2^31. */
 int agh_layer_norm_f32(const void *x, const void *weight, const void *bias, float eps, void *y, void *mean, void *rstd,
                        int64_t rows, int64_t cols);

@@ -55,6 +55,16 @@ def test_rows_of_one_value(ag, dtype, cols):  # noqa: F811
 
 @gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_long_rows_of_one_value(ag, dtype):  # noqa: F811
+    """As above at the most columns that are promised: a thread adds 2048 of them one after another and 16 sums more, 2064^2 u < 1/2."""
+    cols = 2**21
+    x = as_type(np.repeat(np.array([[1000.1], [-7.3e5], [0.1]]), cols, 1), dtype)
+    y, mean, _ = ag.Tensor.from_array(x[0]).layer_norm(stats=True)
+    assert np.array_equal(values_of(mean), x[1][:, 0]) and not values_of(y).any()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("cols", COLS[2:])
 def test_mean_of_rows_far_from_zero(ag, dtype, cols):  # noqa: F811
     """Where the spread is small against the mean, the mean is the rounded one: off by u |mean| and by the f32 sum of the deviations from a first one, (L + 3) u mean |d|,
