@@ -52,6 +52,12 @@ int choose_form(bool gated, int64_t m, int64_t n, int64_t steps, size_t element)
     return best;
 }
 
+// AGH_I8_FORM, an override for experiments: the number of a form that every product takes, few rows too; -1 where it is not set
+int forced_form() {
+    const char *s = setting("AGH_I8_FORM");
+    return s && *s ? atoi(s) : -1;
+}
+
 // Whether x's rows are quantised in the product's launch, by every workgroup again (agh_i8_rows.h), instead of by a launch of its own (one / two, bf16: 1x4096x4096 5.9 /
 // 9.8 us, 1x16384x4096 15.8 / 30, 4x1000x16000 6.7 / 8.3, 16x1000x2000 6.3 / 6.9, 16x4096x4096 12.0 / 10.4; f32: 1x8192x8192 15.3 / 24.3, 16x1000x2000 9.4 / 7.9).  Its codes lie
 // in LDS.
@@ -104,7 +110,9 @@ struct Launch {
     }
     template <bool GATED>
     int run() {
-        switch (choose_form(GATED, p.m, p.n, p.steps, sizeof(T))) {
+        const int forced = forced_form();
+        if (forced >= kFormCount) return fail(AGH_EINVAL, "%s: AGH_I8_FORM=%d: no such form", name, forced);
+        switch (forced >= 0 ? forced : choose_form(GATED, p.m, p.n, p.steps, sizeof(T))) {
             case 0: return direct<GATED, 1, 1, 8, 4>();
             case 1: return direct<GATED, 1, 2, 8, 4>();
             case 2: return direct<GATED, 2, 2, 4, 2>();
@@ -153,7 +161,7 @@ int product(const char *name, int64_t m, int64_t k, int64_t n, const void *a_cod
         if constexpr (GATED)
             if (int rc = check_operand(name, "up", b2_codes, b2_scales)) return rc;
         if (x) {
-            if (csx == 1 && quantises_itself(m, k, sizeof(T))) {
+            if (csx == 1 && forced_form() < 0 && quantises_itself(m, k, sizeof(T))) {
                 // few rows: quantised by every workgroup for itself, in one launch
                 l.x = x;
                 l.rsx = rsx;
