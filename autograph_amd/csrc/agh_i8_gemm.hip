@@ -125,9 +125,10 @@ struct Launch {
     int few() {
         // Two tiles a workgroup where that leaves more than one a CU: half as many quantise the rows (one tile / two, bf16: 1x4096x16384 16.0 / 13.7 us, 4x1000x16000 8.1 / 6.7;
         // 1x8192x8192 15.0 / 16.4, and gated, which is two tiles already, 1x4096x16384 28.1 / 28.5)
-        const bool wide = !GATED && p.n > 3 * 16 * compute_units();
-        if (p.m == 1) return wide ? rows<GATED, 1, 2>() : rows<GATED, 1, 1>();
-        if (p.m <= 4) return wide ? rows<GATED, 4, 2>() : rows<GATED, 4, 1>();
+        if constexpr (!GATED)
+            if (p.m <= 4 && p.n > 3 * 16 * compute_units()) return p.m == 1 ? rows<GATED, 1, 2>() : rows<GATED, 4, 2>();
+        if (p.m == 1) return rows<GATED, 1, 1>();
+        if (p.m <= 4) return rows<GATED, 4, 1>();
         return rows<GATED, 16, 1>();
     }
 };

@@ -3,6 +3,8 @@ large products take by themselves.
 
 Tolerances as in test_int8: sums are exact; their conversion, the scales' product, the product of both and the bias's addition are four roundings of 2^-24 each, the result half a
 step of its type.  A gate's slope is at most 1.13, and gated.gate_error says what the gate adds."""
+import re
+
 import numpy as np
 import pytest
 
@@ -61,6 +63,13 @@ class Result:
 def operands(rng, m, n, k, dtype):
     return (as_type(rng.standard_normal((m, k)) * np.exp2(rng.integers(-6, 6, (m, 1))), dtype), as_type(rng.standard_normal((k, n)) / np.sqrt(k), dtype),
             as_type(rng.standard_normal((n, 2)), dtype))
+
+
+def test_no_kernel_that_nothing_launches():
+    """A gated product of few rows takes one tile of each half a workgroup, never two: the library holds no kernel for that."""
+    from autograph_amd import _ffi
+    names = set(re.findall(rb"i8_rows_kernelI[ft]Lb([01])ELi(\d+)ELi(\d+)E", open(_ffi.lib._name, "rb").read()))
+    assert names == {(b"0", rows, tiles) for rows, tiles in ((b"1", b"1"), (b"1", b"2"), (b"4", b"1"), (b"4", b"2"), (b"16", b"1"))} | {(b"1", rows, b"1") for rows in (b"1", b"4", b"16")}
 
 
 # steps of 64 along k: 1, 3, 4, 5, 9, 11, 18 and 1, so that the four stages are filled in part, once, and several times with each remainder
