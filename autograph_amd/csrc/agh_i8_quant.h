@@ -18,11 +18,12 @@ struct RowScale {
     float most, inv;  // the largest magnitude and its reciprocal, of x * up
     float times;      // 127 up: up = 2^100 where the reciprocal would pass f32 or the remainder lose its last bits, 2^-60 where 127 x would pass it, else 1
     float scale;      // most / 127, or NaN for a row that holds an infinity or a NaN: it stands for NaNs
+                      // (of f32's largest value the f32 below that quotient: 127 times the nearest one is infinity)
     uint32_t keep;    // of the codes: none of such a row
     __device__ __forceinline__ explicit RowScale(uint32_t bits) {
         const bool bad = bits >= 0x7F800000u;
         const float m = bad ? 0.0f : __uint_as_float(bits), up = m < 0x1p-90f ? 0x1p100f : m > 0x1p90f ? 0x1p-60f : 1.0f;
-        scale = bad ? __uint_as_float(0x7FC00000u) : m / 127.0f;
+        scale = bad ? __uint_as_float(0x7FC00000u) : fminf(m / 127.0f, 0x1.020406p+121f);
         keep = bad ? 0u : 0xFFFFFFFFu;
         most = m * up;
         inv = most > 0.0f ? 1.0f / most : 0.0f;  // (a row of zeros: codes 0)

@@ -495,7 +495,9 @@ int agh_dense_mxfp4_bf16(int64_t m, int64_t k, int64_t n, const void *x, int64_t
  * channel of a weight.  No counterpart in the reference; as with MXFP4, what `Tensor::dot` (src/tensor/linalg.rs:410-421) and `Dense`
  * (layer.rs:1134-1143) do, on operands of half of bf16's size.  A value stands for code * scale:
  *   scale = max |x| / 127 (f32), code = 127 x / max |x| to the nearest whole number, half to even, the maximum over the row
- * A row that holds an infinity or a NaN gets the scale NaN: it stands for NaNs.  A row of zeros gets the scale 0.
+ * A row that holds an infinity or a NaN gets the scale NaN: it stands for NaNs.  A row of zeros gets the scale 0.  At the ends of f32: a row whose largest magnitude is f32's
+ * largest value gets the f32 below that quotient, 0x1.020406p+121, since 127 times the nearest is infinity; below 127 * 2^-126 the scale is subnormal and has fewer bits, and
+ * below 2^-143 it is 0, so that such a row stands for zeros, whatever its codes.
  *
  * A matrix of `rows` rows of k values takes two buffers whose sizes agh_int8_bytes says:
  *   codes   16-byte aligned: the 16 codes of row r, chunk b (of 16 along k) are the 16 bytes at ((r / 16 * steps + b / 4) * 64 + b % 4 * 16 + r % 16) * 16,
