@@ -65,7 +65,7 @@ __global__ __launch_bounds__(W * 64) void gated_backward_kernel(const T *h, cons
 #pragma unroll
                 for (int e = 0; e < VE; ++e) {
                     const float d = Group<T>::get(vd[i], e);
-                    dg[e] = d * Group<T>::get(vu[i], e) * dg[e];
+                    dg[e] = d * dg[e] * Group<T>::get(vu[i], e);  // (the slope first: d u alone may pass f32 where it is 0 or small)
                     du[e] = d * du[e];
                     sg[e] += dg[e];
                     su[e] += du[e];

@@ -1,0 +1,41 @@
+"""The gated layer where products of its factors leave f32 and the gradient does not."""
+import numpy as np
+import pytest
+
+import gated as gt
+from test_int8 import STEP, as_type, values_of
+from test_int8_tiles import ACT
+
+gpu = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ag():
+    import autograph_amd as ag
+    ag.Device(0)
+    return ag
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m", [1, 40, 300])
+@pytest.mark.parametrize("n", [3, 130])
+def test_gradients_whose_factors_pass_f32(ag, dtype, m, n):
+    """dy u beyond f32 under a slope that is 0 (relu's gate below 0) or small (silu, gelu and sigmoid far below 0): dg is a number, and so are the sums of its rows."""
+    rng = np.random.default_rng(n)
+    far = {"relu": -2.0, "silu": -50.0, "gelu": -7.0, "sigmoid": -50.0}
+    for activation, g in far.items():
+        slope = abs(float(gt.gate(g, activation)[1]))
+        big = 1e25 if slope == 0 else np.sqrt(1e30 / slope)  # dy u slope of 1e30, its sums of 1e33 at most
+        h = as_type(np.concatenate((np.full((m, n), g), big * rng.uniform(0.5, 1, (m, n))), 1), dtype)
+        dy = as_type(big * rng.uniform(0.5, 1, (m, n)), dtype)
+        assert np.all(dy[1] * h[1][:, n:] > 3.5e38)
+        want = gt.input_grad(h[1], dy[1], activation)
+        th, td, dh, db = ag.Tensor.from_array(h[0]), ag.Tensor.from_array(dy[0]), ag.Tensor.zeros((m, 2 * n), dtype), ag.Tensor.zeros((2 * n,), dtype)
+        call = getattr(ag.lib, f"agh_gated_dense_backward_{dtype}")
+        ag._ffi.check(call(m, 1, n, None, 0, 1, 1, None, 0, 1, 1, th._ptr(), td._ptr(), ACT[activation], dh._ptr(), None, None, db._ptr()))
+        got = values_of(dh)
+        assert np.isfinite(got).all() and np.isfinite(values_of(db)).all()
+        # the slope's two terms by gate_error, of which the larger is at most 1.05 times the slope here; their sum, the products
+        e = 1.1 * gt.gate_error(np.float64(g), activation) + 2.0**-21
+        assert np.all(np.abs(got - want) <= (e + STEP[dtype] * 1.02) * np.abs(want))
