@@ -405,8 +405,8 @@ int gemm_entry(const char *name, int64_t m, int64_t k, int64_t n, float alpha, c
 
     int lp = k > 0 ? pick_loader<T>(g.P, g.ps, g.pk, g.NP, g.K) : LD_S;
     int lq = k > 0 ? pick_loader<T>(g.Q, g.qs, g.qk, g.NQ, g.K) : LD_S;
-    // a gated layer's tile takes rows of both halves of the weight: the second's start on 16 bytes too
-    if (gated && lp == LD_R && g.NP / 2 % EPC != 0) lp = LD_S;
+    // a gated layer's bf16 tile takes rows of both halves of the weight: the second's start on 16 bytes too (f32 multiplies the weight as a whole)
+    if (gated && sizeof(T) == 2 && lp == LD_R && g.NP / 2 % EPC != 0) lp = LD_S;
     // every matrix of a batch must satisfy the same alignment as the first
     const bool batch_aligned = batch == 1 || (g.batch_p % EPC == 0 && g.batch_q % EPC == 0);
     if (!batch_aligned) lp = lq = LD_S;

@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 
 import gated as gt
+from test_gated import check_forward
 from test_int8 import STEP, as_type, values_of
 from test_int8_tiles import ACT
 
@@ -39,3 +40,18 @@ def test_gradients_whose_factors_pass_f32(ag, dtype, m, n):
         # the slope's two terms by gate_error, of which the larger is at most 1.05 times the slope here; their sum, the products
         e = 1.1 * gt.gate_error(np.float64(g), activation) + 2.0**-21
         assert np.all(np.abs(got - want) <= (e + STEP[dtype] * 1.02) * np.abs(want))
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k", [(300, 130, 512), (1000, 1002, 48), (40, 2050, 304), (513, 66, 64), (8, 34, 4), (700, 666, 1000)])
+def test_f32_halves_off_16_bytes(ag, m, n, k):
+    """Rows of the weight on 16 bytes whose second halves are not: f32 reads them in vectors all the same, a row at a time, column by column and through a view."""
+    rng = np.random.default_rng(n)
+    x, w, bias = rng.standard_normal((m, k)).astype(np.float32), rng.standard_normal((k, 2 * n)).astype(np.float32), rng.standard_normal(2 * n).astype(np.float32)
+    layer = ag.GatedDense(ag.Tensor.from_array(w), ag.Tensor.from_array(bias), "silu")
+    for tx in (ag.Tensor.from_array(x), ag.Tensor.from_array(np.ascontiguousarray(x.T)).t()):
+        y, h = layer.forward_train(tx)
+        check_forward(values_of(y), values_of(h), x.astype(np.float64), w.astype(np.float64), bias.astype(np.float64), "silu", "f32")
+    wide = ag.Tensor.from_array(np.concatenate((w, w), 0)).slice_rows(k, 2 * k)
+    y, h = ag.Tensor.from_array(x).gated_dot(wide, None, "gelu", keep=True)
+    check_forward(values_of(y), values_of(h), x.astype(np.float64), w.astype(np.float64), None, "gelu", "f32")
