@@ -8,8 +8,9 @@ namespace agh {
 
 inline bool gate_known(int act) { return act >= AGH_ACT_NONE && act <= AGH_ACT_SIGMOID; }
 
-// Results that are rounded to bf16 (FAST) take the hardware's exponential and reciprocal, off by a few steps of f32, 2^-14 of a step of bf16; for f32 the library's
-// exponential and a division that rounds once.
+// Results that are rounded to bf16 (FAST) take the hardware's exponential and reciprocal; for f32 the library's exponential and a division that rounds once.
+// FAST: the rounding of x log2(e) makes e^x about |x| 2^-23 of its size off, 31 steps of f32 at |x| = 85, and the instructions add a few: at most 2^-11 of a step of bf16.
+// Where e^-g passes f32 or its reciprocal is subnormal, g < -87, silu and sigmoid come out as 0 in place of values of less than 2^-119.
 template <bool FAST>
 __device__ __forceinline__ float gate_exp(float x) {
     if constexpr (FAST) return __builtin_amdgcn_exp2f(x * 1.44269504f);
@@ -22,7 +23,8 @@ __device__ __forceinline__ float gate_divide(float a, float b) {
 }
 
 // P(Z <= g) = erfc(-g / sqrt 2) / 2, Z standard normal: through erfc, since 1 + erf would cancel where g is negative.
-// FAST: erfc(x) = t e^(-x^2 + p(t)), x >= 0, t = 1 / (1 + x / 2), p a polynomial of degree 7 fitted to log2(e^(x^2) erfc(x) / t) for x up to 14 (7e-7 of the value in exact
+// FAST: erfc(x) = t e^(-x^2 + p(t)), x >= 0, t = 1 / (1 + x / 2), the form given by Press, Teukolsky, Vetterling and Flannery, Numerical Recipes, 6.2, with a polynomial of our own: p of
+// degree 7, fitted to log2(e^(x^2) erfc(x) / t) for x up to 14 (7e-7 of the value in exact
 // arithmetic; with x^2's rounding 4e-6 up to |g| = 6 and 2e-5 at 13, where the value is 1e-38).  The library's erfcf is three times as long: a gated product of 16384x4096x4096 903 us instead of 756.
 template <bool FAST>
 __device__ __forceinline__ float gate_share(float g) {

@@ -2,8 +2,9 @@
 //
 //   scale = max |x| / 127 over a row, code = 127 x / max |x| to the nearest whole number (agh_i8_quant.h)
 // A row with an infinity or a NaN gets the scale NaN and codes 0: it stands for NaNs.  A row of zeros gets the scale 0.
-// A row is passed over twice, for its largest magnitude and for its codes: once out of memory, and then out of registers or a cache.  Bounded by memory: bf16 16384x4096 along the rows
-// 32.5 us (6.2 TB/s), f32 65; along the columns, k 4096, 46 and 84, where a lane's 16 values of a chunk are as many loads.
+// A row is passed over twice, for its largest magnitude and for its codes: once out of memory, and then out of registers or, where it is longer than a workgroup holds, out of memory again.  Bounded
+// by memory: bf16 16384x4096 along the rows 32.5 us (6.2 TB/s), f32 65; 16384x8192, read twice, 104 and 175; along the columns, k 4096 of 16384, 47 and 90, where a lane's 16 values of a
+// chunk are as many loads.
 #include "agh_i8_quant.h"
 
 using namespace agh;

@@ -5,9 +5,11 @@
 // address arithmetic beyond a scalar addition a load.
 // A wave holds two sets of Q's fragments and one of P's: while step s is multiplied, the reads of step s + 1 go into the other set, and into P's fragment i as soon as
 // row i of the tile is done, spread over the MFMAs.  Behind the barrier early in step s, the stage that step s was read from is refilled.
-// Bounded by power where the result is large: 8192x8192x8192 bf16 371 to 390 us (2.8 to 3.0 PTOP/s), matrix pipes busy 75 % of the cycles at a clock of 1.69 GHz (waves as 2x2 of
-// 128x128 433, tiles of 128x128 496; 16384x4096x4096 205); where it is small, by the LDS reads of a tile of two waves a SIMD and by idle CUs: 1999x2047x1001 f32 9.8, bf16 8.9, eight stages instead
-// of four 0.2 more.  Gated 16384x4096x8192 854 to 880.
+// Bounded by power where the result is large: 8192x8192x8192 bf16 369 to 390 us, call after call (2.8 to 3.0 PTOP/s), matrix pipes busy 75 % of the cycles at a clock of 1.69 GHz (waves as 2x2 of
+// 128x128 433, tiles of 128x128 496; 16384x4096x4096 205); where it is small, by one workgroup a CU: 1999x2047x1001 has 256 tiles of
+// 128x64, four waves each, so that nothing covers a wave's barrier, its six LDS reads a step and its wait for memory: f32 9.6 to 10.4, bf16 8.7 to 9.4, eight stages instead of four 0.2 more.
+// Gated 16384x4096x8192 854 to 880, in 256x256 tiles, whose bf16 form keeps one register in scratch memory in
+// the epilogue (all 256 are in use), read again for each of a wave's columns of tiles.
 //
 // GATED: the tile's BP rows of P are BP / 2 of b (the gate's) and the same BP / 2 of b2; a wave holds the accumulators of both in the same lanes, and the tile of c is BP / 2 wide.
 #pragma once

@@ -545,8 +545,8 @@ int agh_dense_int8_bf16(int64_t m, int64_t k, int64_t n, const void *x, int64_t 
  *   g = x Wg + bg, u = x Wu + bu, y = act(g) * u
  * x [m, k] and w [k, 2 n] have any element strides; w's columns 0 .. n - 1 are Wg, the others Wu, and bias (may be null) holds 2 n values likewise.  act is one of
  * AGH_ACT_*.  y is [m, n] in standard layout; h, where it is not null, receives g and u side by side, [m, 2 n] in standard layout: what the backward call
- * takes.  Sums, bias, activation and product are f32; y and h are rounded once each.  y and h must not overlap the operands.  m, k or n == 0 is allowed
- * (k == 0: g and u are the biases).  Uses the library's workspace: run a call that is to be captured once eagerly, as for a product with split-K. */
+ * takes.  Sums, bias, activation and product are f32; y and h are rounded once each; values of silu, gelu and sigmoid below 2^-119 may come out as 0.  y and h must not overlap the
+ * operands.  m, k or n == 0 is allowed (k == 0: g and u are the biases).  Uses the library's workspace: run a call that is to be captured once eagerly, as for a product with split-K. */
 int agh_gated_dense_f32(int64_t m, int64_t k, int64_t n, const void *x, int64_t off_x, int64_t rsx, int64_t csx, const void *w,
                         int64_t off_w, int64_t rsw, int64_t csw, const void *bias, int64_t off_bias, int64_t bias_stride,
                         int act, void *y, void *h);
