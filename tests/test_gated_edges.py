@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import gated as gt
-from test_gated import check_forward
+from test_gated import check_forward, slope_error
 from test_int8 import STEP, as_type, values_of
 from test_int8_tiles import ACT
 
@@ -55,3 +55,29 @@ def test_f32_halves_off_16_bytes(ag, m, n, k):
     wide = ag.Tensor.from_array(np.concatenate((w, w), 0)).slice_rows(k, 2 * k)
     y, h = ag.Tensor.from_array(x).gated_dot(wide, None, "gelu", keep=True)
     check_forward(values_of(y), values_of(h), x.astype(np.float64), w.astype(np.float64), None, "gelu", "f32")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,n,k", [(7, 3, 20), (40, 130, 33), (65, 515, 40), (300, 259, 64), (1000, 17, 24), (33, 4099, 8)])
+def test_gradients_one_by_one_and_in_place(ag, dtype, m, n, k):
+    """dh in place of h, where a row's last group of columns lies beside what another workgroup writes, and each gradient alone: the bits of the call that forms them all."""
+    rng = np.random.default_rng(m)
+    x, w, h, dy = (ag.Tensor.from_array(as_type(rng.standard_normal(s), dtype)[0]) for s in ((m, k), (k, 2 * n), (m, 2 * n), (m, n)))
+    call = getattr(ag.lib, f"agh_gated_dense_backward_{dtype}")
+    z = lambda *s: ag.Tensor.zeros(s, dtype)  # noqa: E731
+
+    def run(h, dh, dx=None, dw=None, db=None):
+        at = lambda t: None if t is None else t._ptr()  # noqa: E731
+        ag._ffi.check(call(m, k, n, x._ptr(), 0, k, 1, w._ptr(), 0, 2 * n, 1, h._ptr(), dy._ptr(), 2, dh._ptr(), at(dx), at(dw), at(db)))
+        return [None if t is None else t.into_array() for t in (dh, dx, dw, db)]
+    want = run(h, z(m, 2 * n), z(m, k), z(k, 2 * n), z(2 * n))
+    check_dh = gt.input_grad(values_of(h), values_of(dy), "silu")
+    assert np.all(np.abs(values_of(ag.Tensor.from_array(want[0])) - check_dh) <= slope_error(values_of(h), values_of(dy), "silu") + 1.02 * STEP[dtype] * np.abs(check_dh) + 1e-37)
+    same = ag.Tensor.from_array(h.into_array())
+    for got, ref in zip(run(same, same, z(m, k), z(k, 2 * n), z(2 * n)), want):
+        assert np.array_equal(got, ref)
+    for i, one in enumerate((z(m, k), z(k, 2 * n), z(2 * n))):
+        got = run(h, z(m, 2 * n), *[one if i == j else None for j in range(3)])
+        assert np.array_equal(got[0], want[0]) and np.array_equal(got[1 + i], want[1 + i])
+    assert np.array_equal(run(h, z(m, 2 * n))[0], want[0])
